@@ -254,6 +254,55 @@ int lb_peer_flag_words(void);
 int lb_peer_allreduce(const float *const *bufs, unsigned int *const *flags, int rank, int world, float *out, int64_t n,
                       void *stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * What surrounds a shared block between two reads. These have no counterpart in the reference's fused module: its models
+ * run them as separate PyTorch operations (looped_transformer.py, the block between the reads).
+ * Rows as above (n_tok rows of d elements of `dtype`); wdtype = the storage type of per-channel parameters: `dtype` or
+ * LB_DTYPE_F32. Any gradient output may be NULL (not wanted); n_tok may be 0 (parameter gradients are then zero).
+ * ------------------------------------------------------------------------------------------------------------------ */
+
+/* Bytes of `scratch` for the two backwards below at row width d (a stream's calls may share one buffer). */
+size_t lb_block_scratch_bytes(int d);
+
+/* u = w x r, r = rsqrt(mean(x^2) + eps); r [n_tok] is stored when non-NULL (the backward wants it). */
+int lb_norm_fwd(const void *x, const void *w, void *u, float *r, int64_t n_tok, int d, float eps, int dtype, int wdtype,
+                void *stream);
+
+/* dx = r (w du - xh mean(w du xh)), dw = sum over the rows of du xh, xh = r x. dw is the same bits on every run. */
+int lb_norm_bwd(const void *x, const void *w, const float *r, const void *du, void *dx, void *dw, void *scratch,
+                int64_t n_tok, int d, int dtype, int wdtype, void *stream);
+
+#define LB_GATE_NONE 0
+#define LB_GATE_TOKEN 1    /* [n_tok], dtype */
+#define LB_GATE_CHANNEL 2  /* [d], wdtype */
+#define LB_GATE_FULL 3     /* [n_tok][d], dtype */
+
+/* out = x + s gate m b with b = w y r_y (r_y = rsqrt(mean(y^2) + eps)), or b = y where w is NULL; with next_w also
+ * u = next_w out r_o (r_o = rsqrt(mean(out^2) + eps), taken before out is rounded).
+ *   s          *scale_dev (device, fp32) or, where that is NULL, `scale`
+ *   m          dropout: element e (row-major) takes half e % 8 of the four words of Philox4x32-10 with counter
+ *              (e / 8, offset) and key seed; it is kept, times 65536 / (65536 - threshold), where those 16 bits are at
+ *              least `threshold` (0..65535; 0 = no dropout), else 0 takes its place. rng = device (seed, offset), or NULL: the
+ *              two arguments. rng_used [2] (or NULL) receives the pair, for a backward that runs after rng has moved on.
+ *   r_y, r_o   [n_tok] stored when non-NULL (the backward wants r_y with w, r_o with next_w) */
+int lb_residual_fwd(const void *x, const void *y, const void *w, const void *gate, int gate_kind, const float *scale_dev,
+                    float scale, const void *next_w, void *out, void *u, float *r_y, float *r_o, int threshold,
+                    const int64_t *rng, int64_t seed, int64_t offset, int64_t *rng_used, int64_t n_tok, int d, float eps,
+                    int dtype, int wdtype, void *stream);
+
+/* Gradients of the above for the upstream gradients d_out and d_u (either may be NULL; d_u needs next_w). out is formed
+ * again from x and y. dgate has the gate's shape and type, dscale is one fp32. Parameter gradients are the same bits on
+ * every run. */
+int lb_residual_bwd(const void *x, const void *y, const void *w, const void *gate, int gate_kind, const float *scale_dev,
+                    float scale, const void *next_w, const float *r_y, const float *r_o, int threshold, const int64_t *rng,
+                    int64_t seed, int64_t offset, const void *d_out, const void *d_u, void *dx, void *dy, void *dw,
+                    void *dgate, float *dscale, void *dnext_w, void *scratch, int64_t n_tok, int d, int dtype, int wdtype,
+                    void *stream);
+
+/* out = m x over n_elem elements, m as above: forward, and backward with the gradient in place of x. Not in place. */
+int lb_dropout(const void *x, void *out, int threshold, const int64_t *rng, int64_t seed, int64_t offset, int64_t *rng_used,
+               int64_t n_elem, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

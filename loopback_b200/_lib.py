@@ -51,6 +51,14 @@ SYMBOLS = {
                                   _vp, _vp, _i, _i, _f, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
     "lb_peer_flag_words": (_i, []),
     "lb_peer_allreduce": (_i, [_vp, _vp, _i, _i, _vp, _i64, _vp]),
+    "lb_block_scratch_bytes": (ctypes.c_size_t, [_i]),
+    "lb_norm_fwd": (_i, [_vp, _vp, _vp, _vp, _i64, _i, _f, _i, _i, _vp]),
+    "lb_norm_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _vp]),
+    "lb_residual_fwd": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _f, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i64, _i64, _vp, _i64, _i, _f,
+                             _i, _i, _vp]),
+    "lb_residual_bwd": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _f, _vp, _vp, _vp, _i, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
+                             _vp, _vp, _vp, _i64, _i, _i, _i, _vp]),
+    "lb_dropout": (_i, [_vp, _vp, _i, _vp, _i64, _i64, _vp, _i64, _i, _vp]),
     "lb_read_bwd_noalloc": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i,
                                  _i, _i, _vp]),
 }
@@ -97,7 +105,7 @@ def stream_ptr(device=None):
 # of its query-gradient partials); read by the benchmark
 LAUNCHES = {"count": 0}
 _KERNELS_PER_CALL = {"read backward": 2, "read backward (final)": 2, "combine backward": 2, "step backward": 2,
-                     "step backward (deferred)": 2}
+                     "step backward (deferred)": 2, "block norm backward": 2, "block residual backward": 2}
 
 
 def check(rc: int, what: str) -> None:

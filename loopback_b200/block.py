@@ -1,0 +1,279 @@
+"""What a shared block needs around and inside it, between two reads of the update stack: the norms before and after the
+block with its gate, dropout and residual scale, dropout on its own, and the gated feed-forward product.
+
+    block_norm      u = w n(x),  n(v) = v / sqrt(mean(v^2) + eps)
+    block_residual  out = x + s g m b, with b = w n(y) (or y); and, given the next block's norm, u = w' n(out)
+    dropout         out = m x
+
+The read cell forms a block's input (cell.combine), the caller's block turns it into a proposal with these operators, and
+`DattnStack.write` stores the difference: h = block_residual(x, f(block_norm(x, w)), ...) is what `write(s, h, x)` and
+`combine(h, ...)` take.  Rows are bf16 or fp32 as everywhere in this package, arithmetic is fp32 with one rounding per
+result, and there is no CPU or eager path: inputs the kernels cannot take raise.  The reference's models run these as
+separate PyTorch operations between their reads (looped_transformer.py, the block the reads sit between).
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import check, dtype_code, stream_ptr
+from .fused_dattn import _on, _require_cuda
+
+__all__ = ["block_norm", "block_residual", "dropout"]
+
+GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_FULL = range(4)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _require_rows(x, what):
+    _require_cuda(x, what)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise RuntimeError(f"loopback_b200.{what}: rows need a last dimension of at least one column, got shape {tuple(x.shape)}")
+
+
+def _same_device(what, ref, *tensors):
+    for t in tensors:
+        if t is not None and t.device != ref.device:
+            raise RuntimeError(f"loopback_b200.{what}: a tensor is on {t.device}, the rows are on {ref.device}")
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _scratch(d, dev):
+    return torch.empty(int(_lib.lib().lb_block_scratch_bytes(d)), dtype=torch.uint8, device=dev)
+
+
+def _channel_params(what, x, d, *params):
+    """The per-channel parameters in one storage type the kernels take: the rows' or, where they are fp32 or differ, fp32."""
+    types = {p.dtype for p in params if p is not None}
+    for p in params:
+        if p is not None and p.shape != (d,):
+            raise RuntimeError(f"loopback_b200.{what}: a per-channel parameter has shape {tuple(p.shape)}, rows have {d} columns")
+    if len(types) > 1 or not types <= {x.dtype, torch.float32}:
+        params = tuple(p if p is None else p.float() for p in params)
+    return tuple(p if p is None else p.contiguous() for p in params)
+
+
+# --------------------------------------------------------------------------------------------------------------
+# the norm before a block
+# --------------------------------------------------------------------------------------------------------------
+def _norm_forward(x, w, eps, save):
+    d = x.shape[-1]
+    n_tok = x.numel() // d
+    u = torch.empty_like(x)
+    r = torch.empty(n_tok, dtype=torch.float32, device=x.device) if save else None
+    with _on(x.device):
+        check(_lib.lib().lb_norm_fwd(x.data_ptr(), w.data_ptr(), u.data_ptr(), _p(r), n_tok, d, eps, dtype_code(x.dtype),
+                                     dtype_code(w.dtype), stream_ptr()), "block norm")
+    return u, r
+
+
+class _BlockNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, eps):
+        u, r = _norm_forward(x, w, eps, True)
+        ctx.save_for_backward(x, w, r)
+        return u
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, du):
+        x, w, r = ctx.saved_tensors
+        d = x.shape[-1]
+        du = du.contiguous()
+        dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+        dw = torch.empty_like(w) if ctx.needs_input_grad[1] else None
+        with _on(x.device):
+            scratch = _scratch(d, x.device) if dw is not None else None
+            check(_lib.lib().lb_norm_bwd(x.data_ptr(), w.data_ptr(), r.data_ptr(), du.data_ptr(), _p(dx), _p(dw), _p(scratch),
+                                         x.numel() // d, d, dtype_code(x.dtype), dtype_code(w.dtype), stream_ptr()),
+                  "block norm backward")
+        return dx, dw, None
+
+
+def block_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
+    """weight * x / sqrt(mean(x^2) + eps) over the last dimension, differentiable in both. `weight` (d,) in x's type or
+    fp32."""
+    _require_rows(x, "block_norm")
+    _same_device("block_norm", x, weight)
+    (w,) = _channel_params("block_norm", x, x.shape[-1], weight)
+    x = x.contiguous()
+    if _wants_grad(x, w):
+        return _BlockNorm.apply(x, w, float(eps))
+    return _norm_forward(x, w, float(eps), False)[0]
+
+
+# --------------------------------------------------------------------------------------------------------------
+# dropout
+# --------------------------------------------------------------------------------------------------------------
+def _threshold(what, p):
+    t = int(float(p) * 65536 + 0.5) if 0.0 <= float(p) < 1.0 else -1
+    if not 0 <= t <= 65535:
+        raise ValueError(f"loopback_b200.{what}: need 0 <= p < 1 (to the nearest 1 / 65536), got {p}")
+    return t
+
+
+def _rng_args(what, x, rng):
+    """(device pair or None, seed, offset)"""
+    if isinstance(rng, torch.Tensor):
+        if rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
+            raise RuntimeError(f"loopback_b200.{what}: rng must be a contiguous int64 tensor (seed, offset) or a pair of integers")
+        _same_device(what, x, rng)
+        return rng, 0, 0
+    if rng is None:
+        raise ValueError(f"loopback_b200.{what}: dropout needs rng = (seed, offset)")
+    seed, offset = (int(v) for v in rng)
+    wrap = lambda v: (v & (1 << 64) - 1) - (1 << 64 if v >> 63 & 1 else 0)  # noqa: E731  any 64-bit pattern
+    return None, wrap(seed), wrap(offset)
+
+
+def _dropout_launch(x, threshold, rng, seed, offset, used):
+    out = torch.empty_like(x)
+    with _on(x.device):
+        check(_lib.lib().lb_dropout(x.data_ptr(), out.data_ptr(), threshold, _p(rng), seed, offset, _p(used), x.numel(),
+                                    dtype_code(x.dtype), stream_ptr()), "dropout")
+    return out
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, threshold, rng, seed, offset):
+        used = None if rng is None else torch.empty_like(rng)
+        out = _dropout_launch(x, threshold, rng, seed, offset, used)
+        ctx.save_for_backward(used)
+        ctx.args = threshold, seed, offset
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        (used,) = ctx.saved_tensors
+        threshold, seed, offset = ctx.args
+        return _dropout_launch(g.contiguous(), threshold, used, seed, offset, None), None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, rng) -> torch.Tensor:
+    """Each element is kept with probability 1 - p (p to the nearest 1 / 65536) and scaled by the inverse of what is kept on
+    average, else replaced by 0 (also where it is infinite or NaN). The mask is never stored: the backward draws the same
+    numbers again.
+
+    rng = (seed, offset), two 64-bit integers: a pair of Python integers, or a contiguous int64 tensor of two on x's
+    device, read when the kernel runs (a captured graph draws new numbers on every replay if the offset is advanced in
+    between; the backward uses the pair its forward used). The same pair gives the same mask for the same element count."""
+    _require_cuda(x, "dropout")
+    t = _threshold("dropout", p)
+    pair, seed, offset = _rng_args("dropout", x, rng)
+    x = x.contiguous()
+    if _wants_grad(x):
+        return _Dropout.apply(x, t, pair, seed, offset)
+    return _dropout_launch(x, t, pair, seed, offset, None)
+
+
+# --------------------------------------------------------------------------------------------------------------
+# the end of a block
+# --------------------------------------------------------------------------------------------------------------
+def _wcode(x, w, gate, kind, next_w):
+    for t in (w, next_w, gate if kind == GATE_CHANNEL else None):
+        if t is not None:
+            return dtype_code(t.dtype)
+    return dtype_code(x.dtype)
+
+
+def _residual_forward(x, y, w, gate, scale_t, next_w, kind, scale, eps, threshold, rng, seed, offset, save):
+    d = x.shape[-1]
+    n_tok, dev = x.numel() // d, x.device
+    out = torch.empty_like(x)
+    u = torch.empty_like(x) if next_w is not None else None
+    ry = torch.empty(n_tok, dtype=torch.float32, device=dev) if save and w is not None else None
+    ro = torch.empty(n_tok, dtype=torch.float32, device=dev) if save and next_w is not None else None
+    used = torch.empty_like(rng) if save and rng is not None else None
+    with _on(dev):
+        check(_lib.lib().lb_residual_fwd(x.data_ptr(), y.data_ptr(), _p(w), _p(gate), kind, _p(scale_t), scale, _p(next_w),
+                                         out.data_ptr(), _p(u), _p(ry), _p(ro), threshold, _p(rng), seed, offset, _p(used),
+                                         n_tok, d, eps, dtype_code(x.dtype), _wcode(x, w, gate, kind, next_w), stream_ptr()),
+              "block residual")
+    return out, u, ry, ro, used
+
+
+class _BlockResidual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, w, gate, scale_t, next_w, kind, scale, eps, threshold, rng, seed, offset):
+        out, u, ry, ro, used = _residual_forward(x, y, w, gate, scale_t, next_w, kind, scale, eps, threshold, rng, seed, offset,
+                                                 True)
+        ctx.save_for_backward(x, y, w, gate, scale_t, next_w, ry, ro, used)
+        ctx.args = kind, scale, threshold, seed, offset
+        ctx.set_materialize_grads(False)
+        return (out, u) if u is not None else out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_out, g_u=None):
+        x, y, w, gate, scale_t, next_w, ry, ro, used = ctx.saved_tensors
+        kind, scale, threshold, seed, offset = ctx.args
+        none = (None,) * 7
+        if g_out is None and g_u is None:
+            return (None,) * 6 + none
+        d, dev = x.shape[-1], x.device
+        g_out = None if g_out is None else g_out.contiguous()
+        g_u = None if g_u is None else g_u.contiguous()
+        grads = [torch.empty_like(t) if t is not None and need else None
+                 for t, need in zip((x, y, w, gate, scale_t, next_w), ctx.needs_input_grad)]
+        dx, dy, dw, dgate, dscale, dnext = grads
+        with _on(dev):
+            sums = dw is not None or dscale is not None or dnext is not None or (dgate is not None and kind == GATE_CHANNEL)
+            scratch = _scratch(d, dev) if sums else None
+            check(_lib.lib().lb_residual_bwd(x.data_ptr(), y.data_ptr(), _p(w), _p(gate), kind, _p(scale_t), scale, _p(next_w),
+                                             _p(ry), _p(ro), threshold, _p(used), seed, offset, _p(g_out), _p(g_u), _p(dx),
+                                             _p(dy), _p(dw), _p(dgate), _p(dscale), _p(dnext), _p(scratch), x.numel() // d, d,
+                                             dtype_code(x.dtype), _wcode(x, w, gate, kind, next_w), stream_ptr()),
+                  "block residual backward")
+        return (*grads, *none)
+
+
+def block_residual(x: torch.Tensor, y: torch.Tensor, weight=None, *, gate=None, scale=1.0, next_weight=None,
+                   eps: float = 1e-6, p: float = 0.0, rng=None):
+    """The end of a block in one pass over its rows: out = x + scale * gate * dropout(norm(y)), and, given `next_weight`, the
+    norm the next block starts with. Returns out, or (out, norm of out).
+
+    x, y         the residual stream and the block's output, one shape and type
+    weight       (d,) of the norm after the block; None: no such norm, y itself is added
+    gate         None, (d,) per channel, (..., 1) per token or x's shape
+    scale        a number, or a tensor of one element (learned)
+    next_weight  (d,) of the norm of out; its statistics come from out before it is rounded to its storage type
+    p, rng       dropout of the (normed) block output, as in `dropout`, drawn over x's elements
+    Per-channel parameters are in x's type or fp32, gates per token or element in x's. Differentiable in every tensor."""
+    _require_rows(x, "block_residual")
+    _same_device("block_residual", x, y, weight, gate, next_weight)
+    if y.shape != x.shape or y.dtype != x.dtype:
+        raise RuntimeError(f"loopback_b200.block_residual: x is {tuple(x.shape)} {x.dtype}, y is {tuple(y.shape)} {y.dtype}")
+    d = x.shape[-1]
+    kind = GATE_NONE
+    if gate is not None:
+        kind = (GATE_CHANNEL if gate.shape == (d,) else GATE_FULL if gate.shape == x.shape else
+                GATE_TOKEN if gate.shape == x.shape[:-1] + (1,) else None)
+        if kind is None:
+            raise RuntimeError(f"loopback_b200.block_residual: a gate of shape {tuple(gate.shape)} is neither per channel, per "
+                               f"token nor per element of {tuple(x.shape)}")
+        if kind != GATE_CHANNEL and gate.dtype != x.dtype:
+            raise RuntimeError(f"loopback_b200.block_residual: a gate per token or element has the rows' type, got {gate.dtype}")
+    w, next_w, channel_gate = _channel_params("block_residual", x, d, weight, next_weight, gate if kind == GATE_CHANNEL else None)
+    gate = channel_gate if kind == GATE_CHANNEL else None if gate is None else gate.contiguous()
+    scale_t = None
+    if isinstance(scale, torch.Tensor):
+        if scale.numel() != 1:
+            raise RuntimeError("loopback_b200.block_residual: a learned scale has one element")
+        _same_device("block_residual", x, scale)
+        scale_t, scale = scale.float(), 1.0
+    t = _threshold("block_residual", p)
+    pair, seed, offset = _rng_args("block_residual", x, rng) if t else (None, 0, 0)
+    x, y = x.contiguous(), y.contiguous()
+    if _wants_grad(x, y, w, gate, scale_t, next_w):
+        return _BlockResidual.apply(x, y, w, gate, scale_t, next_w, kind, float(scale), float(eps), t, pair, seed, offset)
+    out, u = _residual_forward(x, y, w, gate, scale_t, next_w, kind, float(scale), float(eps), t, pair, seed, offset, False)[:2]
+    return out if u is None else (out, u)

@@ -686,5 +686,170 @@ static int read_bwd_impl(const void *V, const float *R, void *dV, float *dR, con
     return e == cudaSuccess ? LB_OK : cuda_fail(e, "lb_read_bwd dq reduction launch");
 }
 
+// ---------------------------------------------------------------------------------------------------------
+// what surrounds a block
+// ---------------------------------------------------------------------------------------------------------
+static int check_block(const char *who, int64_t n_tok, int d, int dtype, int wdtype) {
+    const int rc = check_common(n_tok, d, dtype);
+    if (rc) return rc;
+    if (wdtype != dtype && wdtype != LB_DTYPE_F32)
+        return fail(LB_ERR_ARG, "%s: parameters have the rows' storage type or fp32 (dtype %d, wdtype %d)", who, dtype, wdtype);
+    return LB_OK;
+}
+
+static int check_drop(const char *who, int threshold, const int64_t *rng, const int64_t *rng_used) {
+    if (threshold < 0 || threshold > 65535) return fail(LB_ERR_ARG, "%s: threshold %d outside [0, 65535]", who, threshold);
+    if ((reinterpret_cast<uintptr_t>(rng) & 7u) || (reinterpret_cast<uintptr_t>(rng_used) & 7u))
+        return fail(LB_ERR_ALIGN, "%s: rng and rng_used must be 8-byte aligned", who);
+    return LB_OK;
+}
+
+static lb::DropParams drop_params(int threshold, const int64_t *rng, int64_t seed, int64_t offset, int64_t *rng_used) {
+    lb::DropParams dp;
+    dp.threshold = (unsigned)threshold;
+    dp.keep_scale = (float)(65536.0 / (65536.0 - threshold));
+    dp.rng = reinterpret_cast<const long long *>(rng);
+    dp.seed = seed; dp.offset = offset;
+    dp.rng_used = reinterpret_cast<long long *>(rng_used);
+    return dp;
+}
+
+static size_t block_part_floats(int d) { return 2 * (size_t)kMaxGrid * (size_t)d; }
+
+size_t lb_block_scratch_bytes(int d) {
+    if (d <= 0) return 0;
+    return sizeof(float) * block_part_floats(d) + sizeof(double) * (((size_t)d + 31) / 32) + 16;
+}
+
+// the parts of `scratch`, and zeros for the parameters' gradients of an empty batch
+static int finish_block_bwd(const char *who, lb::BlockParams &p, void *scratch, int dtype, int wdtype, bool residual,
+                            cudaStream_t st) {
+    DeviceInfo di;
+    const int rc = device_info(&di);
+    if (rc) return rc;
+    cudaError_t e = cudaSuccess;
+    if (p.n_tok == 0) {
+        const size_t wb = (size_t)p.d * (wdtype == LB_DTYPE_BF16 ? 2 : 4);
+        if (p.dw) e = cudaMemsetAsync(p.dw, 0, wb, st);
+        if (e == cudaSuccess && p.dw_next) e = cudaMemsetAsync(p.dw_next, 0, wb, st);
+        if (e == cudaSuccess && p.dgate && p.gate_kind == lb::kGateChannel) e = cudaMemsetAsync(p.dgate, 0, wb, st);
+        if (e == cudaSuccess && p.dscale) e = cudaMemsetAsync(p.dscale, 0, sizeof(float), st);
+        return e == cudaSuccess ? LB_OK : cuda_fail(e, who);
+    }
+    p.need_a = p.dw || p.dscale || (p.dgate && p.gate_kind == lb::kGateChannel);
+    if (p.need_a || p.dw_next) {
+        if (!scratch) return fail(LB_ERR_ARG, "%s: parameter gradients need scratch", who);
+        if (!aligned16(scratch)) return fail(LB_ERR_ALIGN, "%s: scratch must be 16-byte aligned", who);
+        p.part = static_cast<float *>(scratch);
+        p.ds_part = reinterpret_cast<double *>(p.part + block_part_floats(p.d));
+        if (p.dscale) p.counter = reinterpret_cast<unsigned *>(p.ds_part + (p.d + 31) / 32);
+    }
+    e = lb::launch_block(dtype, wdtype, residual, true, p, di.sms, st);
+    return e == cudaSuccess ? LB_OK : cuda_fail(e, who);
+}
+
+int lb_norm_fwd(const void *x, const void *w, void *u, float *r, int64_t n_tok, int d, float eps, int dtype, int wdtype,
+                void *stream) {
+    int rc = check_block("lb_norm_fwd", n_tok, d, dtype, wdtype);
+    if (rc) return rc;
+    if (n_tok == 0) return LB_OK;
+    if (!x || !w || !u) return fail(LB_ERR_ARG, "lb_norm_fwd: x, w and u must be non-NULL");
+    if (!aligned16(x) || !aligned16(w) || !aligned16(u)) return fail(LB_ERR_ALIGN, "lb_norm_fwd: x, w and u must be 16-byte aligned");
+    DeviceInfo di;
+    if ((rc = device_info(&di))) return rc;
+    lb::BlockParams p;
+    p.x = x; p.w_next = w; p.u = u; p.r_o = r; p.n_tok = n_tok; p.d = d; p.eps = eps;
+    p.frags = d / (dtype == LB_DTYPE_BF16 ? 8 : 4);
+    const cudaError_t e = lb::launch_block(dtype, wdtype, false, false, p, di.sms, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? LB_OK : cuda_fail(e, "lb_norm_fwd launch");
+}
+
+int lb_norm_bwd(const void *x, const void *w, const float *r, const void *du, void *dx, void *dw, void *scratch,
+                int64_t n_tok, int d, int dtype, int wdtype, void *stream) {
+    const int rc = check_block("lb_norm_bwd", n_tok, d, dtype, wdtype);
+    if (rc) return rc;
+    if (n_tok > 0 && (!x || !w || !r || !du)) return fail(LB_ERR_ARG, "lb_norm_bwd: x, w, r and du must be non-NULL");
+    if (!aligned16(x) || !aligned16(w) || !aligned16(du) || !aligned16(dx))
+        return fail(LB_ERR_ALIGN, "lb_norm_bwd: x, w, du and dx must be 16-byte aligned");
+    lb::BlockParams p;
+    p.x = x; p.w_next = w; p.r_o = const_cast<float *>(r); p.d_u = du; p.dx = dx; p.dw_next = dw; p.n_tok = n_tok; p.d = d;
+    p.frags = d / (dtype == LB_DTYPE_BF16 ? 8 : 4);
+    return finish_block_bwd("lb_norm_bwd", p, scratch, dtype, wdtype, false, static_cast<cudaStream_t>(stream));
+}
+
+static int check_gate(const char *who, const void *gate, int kind) {
+    if (kind < LB_GATE_NONE || kind > LB_GATE_FULL) return fail(LB_ERR_ARG, "%s: unknown gate kind %d", who, kind);
+    if ((kind != LB_GATE_NONE) != (gate != nullptr)) return fail(LB_ERR_ARG, "%s: gate and gate_kind do not agree", who);
+    if (kind >= LB_GATE_CHANNEL && !aligned16(gate)) return fail(LB_ERR_ALIGN, "%s: gate must be 16-byte aligned", who);
+    return LB_OK;
+}
+
+int lb_residual_fwd(const void *x, const void *y, const void *w, const void *gate, int gate_kind, const float *scale_dev,
+                    float scale, const void *next_w, void *out, void *u, float *r_y, float *r_o, int threshold,
+                    const int64_t *rng, int64_t seed, int64_t offset, int64_t *rng_used, int64_t n_tok, int d, float eps,
+                    int dtype, int wdtype, void *stream) {
+    int rc = check_block("lb_residual_fwd", n_tok, d, dtype, wdtype);
+    if (rc || (rc = check_drop("lb_residual_fwd", threshold, rng, rng_used))) return rc;
+    if (n_tok == 0) return LB_OK;
+    if ((rc = check_gate("lb_residual_fwd", gate, gate_kind))) return rc;
+    if (!x || !y || !out || (next_w && !u)) return fail(LB_ERR_ARG, "lb_residual_fwd: x, y, out (and u with next_w) must be non-NULL");
+    if (!aligned16(x) || !aligned16(y) || !aligned16(w) || !aligned16(next_w) || !aligned16(out) || !aligned16(u))
+        return fail(LB_ERR_ALIGN, "lb_residual_fwd: rows and weights must be 16-byte aligned");
+    DeviceInfo di;
+    if ((rc = device_info(&di))) return rc;
+    lb::BlockParams p;
+    p.x = x; p.y = y; p.w = w; p.gate = gate; p.gate_kind = gate_kind; p.scale_dev = scale_dev; p.scale = scale; p.w_next = next_w;
+    p.out = out; p.u = u; p.r_y = r_y; p.r_o = r_o; p.n_tok = n_tok; p.d = d; p.eps = eps;
+    p.drop = drop_params(threshold, rng, seed, offset, rng_used);
+    p.frags = d / (dtype == LB_DTYPE_BF16 ? 8 : 4);
+    const cudaError_t e = lb::launch_block(dtype, wdtype, true, false, p, di.sms, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? LB_OK : cuda_fail(e, "lb_residual_fwd launch");
+}
+
+int lb_residual_bwd(const void *x, const void *y, const void *w, const void *gate, int gate_kind, const float *scale_dev,
+                    float scale, const void *next_w, const float *r_y, const float *r_o, int threshold, const int64_t *rng,
+                    int64_t seed, int64_t offset, const void *d_out, const void *d_u, void *dx, void *dy, void *dw,
+                    void *dgate, float *dscale, void *dnext_w, void *scratch, int64_t n_tok, int d, int dtype, int wdtype,
+                    void *stream) {
+    int rc = check_block("lb_residual_bwd", n_tok, d, dtype, wdtype);
+    if (rc || (rc = check_drop("lb_residual_bwd", threshold, rng, nullptr))) return rc;
+    if (n_tok > 0) {
+        if ((rc = check_gate("lb_residual_bwd", gate, gate_kind))) return rc;
+        if (!x || !y || (!d_out && !d_u)) return fail(LB_ERR_ARG, "lb_residual_bwd: x, y and an upstream gradient must be non-NULL");
+        if ((d_u && (!next_w || !r_o)) || (w && !r_y)) return fail(LB_ERR_ARG, "lb_residual_bwd: a norm's backward needs its weight and row scales");
+    }
+    if ((dw && !w) || (dnext_w && !next_w) || (dgate && gate_kind == LB_GATE_NONE) || (dscale && !scale_dev))
+        return fail(LB_ERR_ARG, "lb_residual_bwd: a gradient is wanted of a parameter that is not there");
+    if (!aligned16(x) || !aligned16(y) || !aligned16(w) || !aligned16(next_w) || !aligned16(d_out) || !aligned16(d_u) ||
+        !aligned16(dx) || !aligned16(dy) || (gate_kind == LB_GATE_FULL && !aligned16(dgate)))
+        return fail(LB_ERR_ALIGN, "lb_residual_bwd: rows and weights must be 16-byte aligned");
+    lb::BlockParams p;
+    p.x = x; p.y = y; p.w = w; p.gate = gate; p.gate_kind = gate_kind; p.scale_dev = scale_dev; p.scale = scale; p.w_next = next_w;
+    p.r_y = const_cast<float *>(r_y); p.r_o = const_cast<float *>(r_o); p.d_out = d_out; p.d_u = d_u;
+    p.dx = dx; p.dy = dy; p.dw = dw; p.dgate = dgate; p.dscale = dscale; p.dw_next = dnext_w; p.n_tok = n_tok; p.d = d;
+    p.drop = drop_params(threshold, rng, seed, offset, nullptr);
+    p.frags = d / (dtype == LB_DTYPE_BF16 ? 8 : 4);
+    if (!d_u) p.dw_next = nullptr;
+    rc = finish_block_bwd("lb_residual_bwd", p, scratch, dtype, wdtype, true, static_cast<cudaStream_t>(stream));
+    if (rc || d_u || !dnext_w) return rc;
+    const cudaError_t e = cudaMemsetAsync(dnext_w, 0, (size_t)d * (wdtype == LB_DTYPE_BF16 ? 2 : 4), static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? LB_OK : cuda_fail(e, "lb_residual_bwd");
+}
+
+int lb_dropout(const void *x, void *out, int threshold, const int64_t *rng, int64_t seed, int64_t offset, int64_t *rng_used,
+               int64_t n_elem, int dtype, void *stream) {
+    if (dtype != LB_DTYPE_BF16 && dtype != LB_DTYPE_F32) return fail(LB_ERR_ARG, "bad dtype %d", dtype);
+    if (n_elem < 0) return fail(LB_ERR_ARG, "lb_dropout: negative size");
+    int rc = check_drop("lb_dropout", threshold, rng, rng_used);
+    if (rc) return rc;
+    if (n_elem > 0 && (!x || !out || x == out)) return fail(LB_ERR_ARG, "lb_dropout: x and out must be non-NULL and two buffers");
+    if (!aligned16(x) || !aligned16(out)) return fail(LB_ERR_ALIGN, "lb_dropout: x and out must be 16-byte aligned");
+    DeviceInfo di;
+    if ((rc = device_info(&di))) return rc;
+    const cudaError_t e = lb::launch_dropout(dtype, x, out, n_elem, drop_params(threshold, rng, seed, offset, rng_used), di.sms,
+                                             static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? LB_OK : cuda_fail(e, "lb_dropout launch");
+}
+
 }  // extern "C"
 #pragma GCC visibility pop

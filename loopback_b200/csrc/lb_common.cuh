@@ -195,6 +195,9 @@ template <> struct Store<__nv_bfloat16> {
     }
     // the value a store of `x` would hold, back in fp32
     __device__ __forceinline__ static float round(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
+    // one element
+    __device__ __forceinline__ static float load1(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+    __device__ __forceinline__ static void store1(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
 
     // the same fragment as element PAIRS, the operand shape of the packed fp32 instructions (fma.rn.f32x2)
     static constexpr int kPairs = 4;
@@ -234,6 +237,8 @@ template <> struct Store<float> {
                           __float_as_uint(f[3]));
     }
     __device__ __forceinline__ static float round(float x) { return x; }
+    __device__ __forceinline__ static float load1(const float *p) { return *p; }
+    __device__ __forceinline__ static void store1(float *p, float v) { *p = v; }
 
     static constexpr int kPairs = 2;
     __device__ __forceinline__ static void unpack2(const uint4 &u, float2 (&f)[2]) {

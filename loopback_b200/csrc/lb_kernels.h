@@ -180,4 +180,41 @@ struct PeerReduceParams {
 int peer_allreduce_ctas(long long n4);
 cudaError_t launch_peer_allreduce(PeerReduceParams p, cudaStream_t stream);
 
+// What surrounds a block: norms, gate, dropout, residual scale (lb_block.cu)
+struct DropParams {
+    unsigned threshold = 0;            // an element is kept where its 16-bit number is at least this; 0 = no dropout
+    float keep_scale = 1.f;            // 65536 / (65536 - threshold)
+    const long long *rng = nullptr;    // device: (seed, offset), or null: the two values below
+    long long seed = 0, offset = 0;
+    long long *rng_used = nullptr;     // [2] receives the pair a forward used, or null
+};
+
+enum GateKind : int { kGateNone = 0, kGateToken = 1, kGateChannel = 2, kGateFull = 3 };
+
+struct BlockParams {
+    const void *x = nullptr, *y = nullptr;         // [n_tok][d] residual stream, block output (y null: a norm on its own)
+    const void *w = nullptr;                       // [d] norm after the block, or null: none
+    const void *gate = nullptr;                    // [n_tok], [d] (weights' type) or [n_tok][d] by gate_kind
+    const void *w_next = nullptr;                  // [d] norm of the result, or null
+    const float *scale_dev = nullptr;              // device scalar, or null: `scale`
+    float scale = 1.f;
+    int gate_kind = kGateNone;
+    DropParams drop;
+    void *out = nullptr, *u = nullptr;             // forward results
+    float *r_y = nullptr, *r_o = nullptr;          // [n_tok] row scales: written by the forward (or null), read by the backward
+    const void *d_out = nullptr, *d_u = nullptr;   // upstream gradients, each may be null
+    void *dx = nullptr, *dy = nullptr, *dw = nullptr, *dgate = nullptr, *dw_next = nullptr;
+    float *dscale = nullptr;
+    float *part = nullptr;                         // [CTAs][2][d] column sums, or null: no parameter wants a gradient
+    double *ds_part = nullptr;                     // [ceil(d / 32)]
+    unsigned *counter = nullptr;
+    long long n_tok = 0;
+    int d = 0, frags = 0, wpt = 1;
+    int need_a = 0;                                // dw, a channel gate's gradient or dscale is wanted
+    float eps = 0.f;
+};
+int block_bwd_rows(int sms);                       // CTAs of the backward at most = rows of `part`
+cudaError_t launch_block(int dtype, int wdtype, bool residual, bool bwd, const BlockParams &p, int sms, cudaStream_t stream);
+cudaError_t launch_dropout(int dtype, const void *x, void *out, long long n, const DropParams &dp, int sms, cudaStream_t stream);
+
 }  // namespace lb
