@@ -62,7 +62,8 @@ int lb_device_error(int clear);
  * tiled write kernel, whatever the batch size; 3: the tensor-core write kernel whatever the batch size),
  * "write_mt" (16-token tiles per consumer warp of the tensor-core write kernel: 1 or 2),
  * "write_tile" (tokens per tile of the tensor-core write kernel: a multiple of 32 up to 256), "write_stages" (its TMA
- * ring depth, 2..8), "fwd_sps" (sources per TMA stage of the forward read: 1, 2 or 4), "wait_cycles" (the limit of
+ * ring depth, 2..8), "fwd_sps" (sources per TMA stage of the forward read: 1, 2 or 4), "ffn_tile" (tile shape of the feed-forward products, 1..: an
+ * index into the shapes they are built for), "ffn_splits" (slices along k, where a product may be split), "wait_cycles" (the limit of
  * every bounded wait inside the kernels, in GPU clock cycles; default 4e9), "test_skip_item" (test hook: the first
  * CTA of the next forward reads leaves out its k-th tile copy, so that a bounded wait runs out, the CTA unwinds and
  * lb_device_error reports it; nothing traps or hangs). Value 0 restores the default
@@ -302,6 +303,33 @@ int lb_residual_bwd(const void *x, const void *y, const void *w, const void *gat
 /* out = m x over n_elem elements, m as above: forward, and backward with the gradient in place of x. Not in place. */
 int lb_dropout(const void *x, void *out, int threshold, const int64_t *rng, int64_t seed, int64_t offset, int64_t *rng_used,
                int64_t n_elem, int dtype, void *stream);
+
+/* The gated feed-forward block: g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T. x, y [n_tok][d]; Wg, Wu [f][d] and
+ * Wd [d][f] (torch's Linear layout); everything bf16, products on the tensor cores with fp32 accumulation, h and y rounded
+ * once each. d and f are multiples of 8. The block is two launches (both projections, the activation and the product in
+ * the first), or three where the second is split along f. */
+#define LB_ACT_SILU 0 /* g / (1 + exp(-g)) */
+#define LB_ACT_GELU 1 /* g (1 + erf(g / sqrt 2)) / 2 */
+
+#define LB_FFN_FORWARD 0
+#define LB_FFN_BACKWARD 1
+
+/* Bytes of `workspace` a call of this size needs on the current device (0 and an error message for sizes it refuses). */
+size_t lb_ffn_workspace_bytes(int64_t n_tok, int d, int f, int kind);
+
+/* Bytes of `kept`: what a forward leaves for the backward besides h, in a layout private to this library (act'(g) u and
+ * act(g) with 24 bits each, 6 bytes per element of h, rows and columns rounded up to 32). */
+size_t lb_ffn_kept_bytes(int64_t n_tok, int f);
+
+/* h [n_tok][f] is written in any case (the backward wants it); kept may be NULL: no backward. */
+int lb_ffn_fwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, void *y, void *h, void *kept,
+               void *workspace, size_t workspace_bytes, int64_t n_tok, int d, int f, int act, int dtype, void *stream);
+
+/* Gradients for the upstream gradient dy [n_tok][d], from the forward's h and kept: dx [n_tok][d]; dw_gate_up [2][f][d], the
+ * gate's then the up projection's; dw_down [d][f]. Any of the three may be NULL. Same bits on every run. */
+int lb_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *h, const void *kept,
+               const void *dy, void *dx, void *dw_gate_up, void *dw_down, void *workspace, size_t workspace_bytes,
+               int64_t n_tok, int d, int f, int dtype, void *stream);
 
 #ifdef __cplusplus
 }

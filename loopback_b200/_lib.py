@@ -59,6 +59,10 @@ SYMBOLS = {
     "lb_residual_bwd": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _f, _vp, _vp, _vp, _i, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
                              _vp, _vp, _vp, _i64, _i, _i, _i, _vp]),
     "lb_dropout": (_i, [_vp, _vp, _i, _vp, _i64, _i64, _vp, _i64, _i, _vp]),
+    "lb_ffn_workspace_bytes": (ctypes.c_size_t, [_i64, _i, _i, _i]),
+    "lb_ffn_kept_bytes": (ctypes.c_size_t, [_i64, _i]),
+    "lb_ffn_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _i64, _i, _i, _i, _i, _vp]),
+    "lb_ffn_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _i64, _i, _i, _i, _vp]),
     "lb_read_bwd_noalloc": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i,
                                  _i, _i, _vp]),
 }
@@ -105,7 +109,8 @@ def stream_ptr(device=None):
 # of its query-gradient partials); read by the benchmark
 LAUNCHES = {"count": 0}
 _KERNELS_PER_CALL = {"read backward": 2, "read backward (final)": 2, "combine backward": 2, "step backward": 2,
-                     "step backward (deferred)": 2, "block norm backward": 2, "block residual backward": 2}
+                     "step backward (deferred)": 2, "block norm backward": 2, "block residual backward": 2,
+                     "gated ffn": 2, "gated ffn backward": 4}
 
 
 def check(rc: int, what: str) -> None:

@@ -4,6 +4,7 @@ block with its gate, dropout and residual scale, dropout on its own, and the gat
     block_norm      u = w n(x),  n(v) = v / sqrt(mean(v^2) + eps)
     block_residual  out = x + s g m b, with b = w n(y) (or y); and, given the next block's norm, u = w' n(out)
     dropout         out = m x
+    gated_ffn       y = (act(x Wg^T) * (x Wu^T)) Wd^T
 
 The read cell forms a block's input (cell.combine), the caller's block turns it into a proposal with these operators, and
 `DattnStack.write` stores the difference: h = block_residual(x, f(block_norm(x, w)), ...) is what `write(s, h, x)` and
@@ -20,7 +21,7 @@ from . import _lib
 from ._lib import check, dtype_code, stream_ptr
 from .fused_dattn import _on, _require_cuda
 
-__all__ = ["block_norm", "block_residual", "dropout"]
+__all__ = ["block_norm", "block_residual", "dropout", "gated_ffn"]
 
 GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_FULL = range(4)
 
@@ -277,3 +278,83 @@ def block_residual(x: torch.Tensor, y: torch.Tensor, weight=None, *, gate=None, 
         return _BlockResidual.apply(x, y, w, gate, scale_t, next_w, kind, float(scale), float(eps), t, pair, seed, offset)
     out, u = _residual_forward(x, y, w, gate, scale_t, next_w, kind, float(scale), float(eps), t, pair, seed, offset, False)[:2]
     return out if u is None else (out, u)
+
+
+# --------------------------------------------------------------------------------------------------------------
+# the gated feed-forward product
+# --------------------------------------------------------------------------------------------------------------
+_ACTS = {"silu": 0, "gelu": 1}
+_FFN_FORWARD, _FFN_BACKWARD = 0, 1
+
+
+def _ffn_workspace(n_tok, d, f, kind, dev):
+    nbytes = int(_lib.lib().lb_ffn_workspace_bytes(n_tok, d, f, kind))
+    if nbytes == 0:
+        raise RuntimeError("loopback_b200.gated_ffn: " + _lib.lib().lb_last_error_string().decode("utf-8", "replace"))
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+
+
+def _ffn_forward(x, wg, wu, wd, act, save):
+    d, f, dev = x.shape[-1], wg.shape[0], x.device
+    n_tok = x.numel() // d
+    y = torch.empty_like(x)
+    h = torch.empty((n_tok, f), dtype=x.dtype, device=dev)
+    with _on(dev):
+        ws = _ffn_workspace(n_tok, d, f, _FFN_FORWARD, dev)
+        kept = torch.empty(int(_lib.lib().lb_ffn_kept_bytes(n_tok, f)), dtype=torch.uint8, device=dev) if save else None
+        check(_lib.lib().lb_ffn_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), h.data_ptr(), _p(kept),
+                                    ws.data_ptr(), ws.numel(), n_tok, d, f, act, dtype_code(x.dtype), stream_ptr()), "gated ffn")
+    return y, h, kept
+
+
+class _GatedFFN(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wg, wu, wd, act):
+        y, h, kept = _ffn_forward(x, wg, wu, wd, act, True)
+        ctx.save_for_backward(x, wg, wu, wd, h, kept)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, wg, wu, wd, h, kept = ctx.saved_tensors
+        d, f, dev = x.shape[-1], wg.shape[0], x.device
+        n_tok = x.numel() // d
+        dy = dy.contiguous()
+        need = ctx.needs_input_grad
+        dx = torch.empty_like(x) if need[0] else None
+        dgu = torch.empty((2, f, d), dtype=x.dtype, device=dev) if need[1] or need[2] else None
+        dwd = torch.empty_like(wd) if need[3] else None
+        with _on(dev):
+            ws = _ffn_workspace(n_tok, d, f, _FFN_BACKWARD, dev)
+            check(_lib.lib().lb_ffn_bwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), h.data_ptr(), kept.data_ptr(),
+                                        dy.data_ptr(), _p(dx), _p(dgu), _p(dwd), ws.data_ptr(), ws.numel(), n_tok, d, f,
+                                        dtype_code(x.dtype), stream_ptr()), "gated ffn backward")
+        return dx, dgu[0] if need[1] else None, dgu[1] if need[2] else None, dwd, None
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, act: str = "silu") -> torch.Tensor:
+    """(act(x w_gate^T) * (x w_up^T)) w_down^T, differentiable in every tensor.
+
+    x (..., d), w_gate and w_up (f, d), w_down (d, f), all bf16 (the products run on the tensor cores in bf16 with fp32
+    accumulation; h and the result, and in the backward the two gradients behind the product, are each rounded once),
+    contiguous weights, d and f multiples of 8. act: "silu" or "gelu" (with erf). Both projections, the activation and the
+    product are one launch. With gradients h and two factors of 24 bits are kept: 8 bytes per token and column of f."""
+    _require_rows(x, "gated_ffn")
+    _same_device("gated_ffn", x, w_gate, w_up, w_down)
+    if act not in _ACTS:
+        raise ValueError(f"loopback_b200.gated_ffn: act is one of {sorted(_ACTS)}, got {act!r}")
+    d = x.shape[-1]
+    if w_gate.dim() != 2 or w_gate.shape[1] != d or w_up.shape != w_gate.shape or w_down.shape != w_gate.shape[::-1]:
+        raise RuntimeError(f"loopback_b200.gated_ffn: rows have {d} columns, weights are {tuple(w_gate.shape)}, "
+                           f"{tuple(w_up.shape)}, {tuple(w_down.shape)}; expected (f, d), (f, d), (d, f)")
+    for t in (x, w_gate, w_up, w_down):
+        if t.dtype != torch.bfloat16:
+            raise RuntimeError(f"loopback_b200.gated_ffn: the products run in bf16, got {t.dtype}")
+    for t in (w_gate, w_up, w_down):
+        if not t.is_contiguous():
+            raise RuntimeError("loopback_b200.gated_ffn: weights must be contiguous")
+    x = x.contiguous()
+    if _wants_grad(x, w_gate, w_up, w_down):
+        return _GatedFFN.apply(x, w_gate, w_up, w_down, _ACTS[act])
+    return _ffn_forward(x, w_gate, w_up, w_down, _ACTS[act], False)[0]

@@ -37,7 +37,8 @@ int cuda_fail(cudaError_t e, const char *what) {
 
 struct Options {
     int fwd_stages = 0, bwd_stages = 0, fwd_fr = 0, grid_cap = 0, fwd_warps = 0, bwd_warps = 0, bwd_wpt = 0,
-        tma_per_chunk = 0, write_tt = 0, write_mt = 0, fwd_sps = 0, write_tile = 0, write_stages = 0, wait_cycles = 0, test_skip_item = 0;
+        tma_per_chunk = 0, write_tt = 0, write_mt = 0, fwd_sps = 0, write_tile = 0, write_stages = 0, wait_cycles = 0, test_skip_item = 0,
+        ffn_tile = 0, ffn_splits = 0;
 } g_opt;
 
 struct DeviceInfo {
@@ -54,6 +55,13 @@ int device_info(DeviceInfo *out) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
     if (dev < 0 || dev >= 64) return fail(LB_ERR_CUDA, "device ordinal %d out of range", dev);
+    // tensor maps are encoded through the driver, which wants a context bound to the calling thread; a thread that has made
+    // no runtime call yet (autograd's, at its first backward) has none
+    static thread_local int bound = -1;
+    if (bound != dev) {
+        if ((e = cudaSetDevice(dev)) != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
+        bound = dev;
+    }
     std::lock_guard<std::mutex> lk(mu);
     if (!cache[dev].ok) {
         DeviceInfo di;
@@ -204,6 +212,8 @@ int lb_set_option(const char *name, int value) {
     else if (!strcmp(name, "write_tile")) g_opt.write_tile = value;
     else if (!strcmp(name, "write_stages")) g_opt.write_stages = value;
     else if (!strcmp(name, "wait_cycles")) g_opt.wait_cycles = value;
+    else if (!strcmp(name, "ffn_tile")) g_opt.ffn_tile = value;
+    else if (!strcmp(name, "ffn_splits")) g_opt.ffn_splits = value;
     else if (!strcmp(name, "test_skip_item")) g_opt.test_skip_item = value;
     else return fail(LB_ERR_ARG, "unknown option '%s'", name);
     return LB_OK;
@@ -849,6 +859,223 @@ int lb_dropout(const void *x, void *out, int threshold, const int64_t *rng, int6
     const cudaError_t e = lb::launch_dropout(dtype, x, out, n_elem, drop_params(threshold, rng, seed, offset, rng_used), di.sms,
                                              static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? LB_OK : cuda_fail(e, "lb_dropout launch");
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// the gated feed-forward block
+// ---------------------------------------------------------------------------------------------------------
+// 2-D bf16 matrix [rows][cols], `ld` columns from row to row; boxes of 64 columns x box_rows rows, 128-byte swizzle
+static int make_map_tile(CUtensorMap *m, const void *base, long long rows, long long cols, long long ld, int box_rows) {
+    auto fn = encode_fn();
+    if (!fn) return fail(LB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(LB_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    return LB_OK;
+}
+
+// the fp32 slices [splits][rows][cols] of a product split along k; boxes of 32 columns x 32 rows
+static int make_map_part(CUtensorMap *m, void *base, long long rows, long long cols, int splits) {
+    auto fn = encode_fn();
+    if (!fn) return fail(LB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)splits};
+    cuuint64_t strides[2] = {(cuuint64_t)cols * 4, (cuuint64_t)cols * 4 * (cuuint64_t)rows};
+    cuuint32_t box[3] = {32, 32, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(LB_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    return LB_OK;
+}
+
+struct GemmPlan {
+    int tile = 0, splits = 1;
+    int m_tiles = 0, n_tiles = 0;
+};
+
+// Tile shape and split along k of an m x n product over `blocks` blocks of 64: the least estimated time.
+static GemmPlan plan_gemm(long long m, long long n, long long blocks, bool gate, bool may_split, int sms) {
+    GemmPlan best;
+    double best_us = 1e30;
+    for (int i = 0; i < lb::kGemmTileCount; ++i) {
+        if (g_opt.ffn_tile > 0 && g_opt.ffn_tile <= lb::kGemmTileCount && g_opt.ffn_tile - 1 != i) continue;
+        const int cg = lb::kGemmTiles[i].cg, bn = lb::kGemmTiles[i].bn;
+        const long long tm = 128LL * cg, tn = gate ? bn / 2 : bn, groups = sms / cg;
+        const long long mt = (m + tm - 1) / tm, nt = (n + tn - 1) / tn;
+        for (int s = 1; s <= 16; ++s) {
+            if (s > 1 && (!may_split || blocks / s < 4)) break;
+            if (may_split && g_opt.ffn_splits > 0 && s != g_opt.ffn_splits) continue;
+            const double waves = (double)((mt * nt * s + groups - 1) / groups);
+            const double rate = (cg == 2 ? 1.0 : bn == 256 ? 1.15 : 1.35) * bn / 256. * 0.41;          // us per block of 64
+            double us = waves * (double)((blocks + s - 1) / s) * rate + 4.0 + bn / 128.;
+            if (s > 1) us += 3.0 + (double)s * m * n * 8. / 4.0e6;                                     // slices out and in
+            if (us < best_us) { best_us = us; best.tile = i; best.splits = s; best.m_tiles = (int)mt; best.n_tiles = (int)nt; }
+        }
+    }
+    return best;
+}
+
+struct Operand {
+    const void *base;
+    long long rows, cols, ld;         // as it lies in memory
+};
+
+// One product m x n over `segs` segments of k columns each. C: `out` [m][n] (ld n), through `part` where k is split.
+static int run_gemm(const char *who, int epi, int form, const GemmPlan &pl, const Operand *a, const Operand *b, const Operand *c,
+                    void *kept, void *part, long long m, long long n, long long k, int segs, int act, const DeviceInfo &di,
+                    cudaStream_t st) {
+    lb::GemmMaps maps;
+    memset(&maps, 0, sizeof maps);
+    lb::GemmParams p;
+    const int cg = lb::kGemmTiles[pl.tile].cg, bn = lb::kGemmTiles[pl.tile].bn;
+    int rc;
+    const bool split = pl.splits > 1;
+    for (int s = 0; s < segs; ++s)
+        if ((rc = make_map_tile(&maps.a[s], a[s].base, a[s].rows, a[s].cols, a[s].ld, form == lb::kFormMN ? 64 : 128))) return rc;
+    for (int s = 0; s < (epi == lb::kEpiGate ? 2 : segs); ++s)
+        if ((rc = make_map_tile(&maps.b[s], b[s].base, b[s].rows, b[s].cols, b[s].ld,
+                                form != lb::kFormKK ? 64 : epi == lb::kEpiGate ? bn / 2 : bn / cg))) return rc;
+    if (split) {
+        if ((rc = make_map_part(&maps.c[0], part, m, n, pl.splits))) return rc;
+    } else {
+        for (int i = 0; i < 2; ++i)
+            if (c[i].base && (rc = make_map_tile(&maps.c[i], c[i].base, c[i].rows, c[i].cols, c[i].ld, 32))) return rc;
+    }
+    p.m = (int)m; p.n = (int)n; p.kblocks = (int)((k + 63) / 64); p.segs = segs;
+    p.m_tiles = pl.m_tiles; p.n_tiles = pl.n_tiles; p.splits = pl.splits; p.act = act; p.kept = static_cast<uint8_t *>(kept);
+    p.err_word = di.err_word; p.wait_cycles = wait_limit();
+    cudaError_t err = lb::launch_gemm(pl.tile, split ? (int)lb::kEpiPartial : epi, form, maps, p, di.sms, st);
+    if (err == cudaSuccess && split)
+        err = lb::launch_gemm_sum(static_cast<const float *>(part), const_cast<void *>(c[0].base), pl.splits, m * n, di.sms, st);
+    return err == cudaSuccess ? LB_OK : cuda_fail(err, who);
+}
+
+struct FfnPlan {
+    GemmPlan up, down, dh, dx, dw_gu, dw_down;
+    size_t part = 0, bytes = 0;                         // offset of the slices in the workspace (dg | du lie before them), its size
+};
+
+static FfnPlan plan_ffn(long long t, long long d, long long f, bool bwd, int sms) {
+    FfnPlan q;
+    const auto blocks = [](long long k) { return (k + 63) / 64; };
+    size_t part = 0;
+    const auto need = [&](const GemmPlan &g, long long m, long long n) {
+        const size_t b = g.splits > 1 ? (size_t)g.splits * (size_t)m * (size_t)n * 4 : 0;
+        if (b > part) part = b;
+    };
+    if (!bwd) {
+        q.up = plan_gemm(t, f, blocks(d), true, false, sms);
+        q.down = plan_gemm(t, d, blocks(f), false, true, sms);
+        need(q.down, t, d);
+    } else {
+        q.dh = plan_gemm(t, f, blocks(d), false, false, sms);
+        q.dx = plan_gemm(t, d, 2 * blocks(f), false, true, sms);
+        q.dw_gu = plan_gemm(2 * f, d, blocks(t), false, true, sms);
+        q.dw_down = plan_gemm(d, f, blocks(t), false, true, sms);
+        need(q.dx, t, d);
+        need(q.dw_gu, 2 * f, d);
+        need(q.dw_down, d, f);
+    }
+    const auto align = [](size_t b) { return (b + 255) / 256 * 256; };
+    q.part = bwd ? align((size_t)t * (size_t)f * 4) : 0;
+    q.bytes = q.part + part;
+    return q;
+}
+
+static int check_ffn(const char *who, int64_t n_tok, int d, int f, int act, int dtype) {
+    if (dtype != LB_DTYPE_BF16) return fail(LB_ERR_UNSUPPORTED, "%s: the products run in bf16 (dtype %d)", who, dtype);
+    if (act != LB_ACT_SILU && act != LB_ACT_GELU) return fail(LB_ERR_ARG, "%s: unknown activation %d", who, act);
+    if (n_tok < 0 || d <= 0 || f <= 0) return fail(LB_ERR_ARG, "%s: n_tok=%lld, d=%d, f=%d: sizes must be positive", who, (long long)n_tok, d, f);
+    if (d % 8 || f % 8) return fail(LB_ERR_ALIGN, "%s: d=%d and f=%d must be multiples of 8 (rows of 16-byte units)", who, d, f);
+    if (d > (1 << 20) || f > (1 << 20) || n_tok >= (1LL << 31) - 512)
+        return fail(LB_ERR_UNSUPPORTED, "%s: n_tok=%lld, d=%d, f=%d exceed the kernels' 32-bit coordinates", who, (long long)n_tok, d, f);
+    return LB_OK;
+}
+
+size_t lb_ffn_workspace_bytes(int64_t n_tok, int d, int f, int kind) {
+    if (check_ffn("lb_ffn_workspace_bytes", n_tok, d, f, LB_ACT_SILU, LB_DTYPE_BF16)) return 0;
+    DeviceInfo di;
+    if (device_info(&di)) return 0;
+    return plan_ffn(n_tok, d, f, kind == LB_FFN_BACKWARD, di.sms).bytes + 16;
+}
+
+size_t lb_ffn_kept_bytes(int64_t n_tok, int f) {
+    if (check_ffn("lb_ffn_kept_bytes", n_tok, 8, f, LB_ACT_SILU, LB_DTYPE_BF16)) return 0;
+    return (size_t)((n_tok + 31) / 32) * (size_t)((f + 31) / 32) * 12 * 512 + 16;
+}
+
+int lb_ffn_fwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, void *y, void *h, void *kept,
+               void *workspace, size_t workspace_bytes, int64_t n_tok, int d, int f, int act, int dtype, void *stream) {
+    const char *who = "lb_ffn_fwd";
+    int rc = check_ffn(who, n_tok, d, f, act, dtype);
+    if (rc) return rc;
+    if (n_tok == 0) return LB_OK;
+    if (!x || !w_gate || !w_up || !w_down || !y || !h || !workspace) return fail(LB_ERR_ARG, "%s: NULL pointer", who);
+    if (!aligned16(x) || !aligned16(w_gate) || !aligned16(w_up) || !aligned16(w_down) || !aligned16(y) || !aligned16(h) ||
+        !aligned16(kept) || !aligned16(workspace))
+        return fail(LB_ERR_ALIGN, "%s: every pointer must be 16-byte aligned", who);
+    DeviceInfo di;
+    if ((rc = device_info(&di))) return rc;
+    const FfnPlan q = plan_ffn(n_tok, d, f, false, di.sms);
+    if (workspace_bytes < q.bytes) return fail(LB_ERR_ARG, "%s: workspace of %zu bytes, %zu are needed", who, workspace_bytes, q.bytes);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    void *part = static_cast<char *>(workspace) + q.part;
+    const Operand xs[1] = {{x, n_tok, d, d}}, w2[2] = {{w_gate, f, d, d}, {w_up, f, d, d}}, hs[2] = {{h, n_tok, f, f}, {}};
+    if ((rc = run_gemm(who, lb::kEpiGate, lb::kFormKK, q.up, xs, w2, hs, kept, nullptr, n_tok, f, d, 1, act, di, st))) return rc;
+    const Operand wd[1] = {{w_down, d, f, f}}, ys[2] = {{y, n_tok, d, d}, {}};
+    return run_gemm(who, lb::kEpiStore, lb::kFormKK, q.down, hs, wd, ys, nullptr, part, n_tok, d, f, 1, act, di, st);
+}
+
+int lb_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *h, const void *kept,
+               const void *dy, void *dx, void *dw_gate_up, void *dw_down, void *workspace, size_t workspace_bytes,
+               int64_t n_tok, int d, int f, int dtype, void *stream) {
+    const char *who = "lb_ffn_bwd";
+    int rc = check_ffn(who, n_tok, d, f, LB_ACT_SILU, dtype);
+    if (rc) return rc;
+    if (!aligned16(x) || !aligned16(w_gate) || !aligned16(w_up) || !aligned16(w_down) || !aligned16(h) || !aligned16(kept) ||
+        !aligned16(dy) || !aligned16(dx) || !aligned16(dw_gate_up) || !aligned16(dw_down) || !aligned16(workspace))
+        return fail(LB_ERR_ALIGN, "%s: every pointer must be 16-byte aligned", who);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (n_tok == 0) {
+        cudaError_t e = cudaSuccess;
+        if (dw_gate_up) e = cudaMemsetAsync(dw_gate_up, 0, (size_t)4 * d * f, st);
+        if (e == cudaSuccess && dw_down) e = cudaMemsetAsync(dw_down, 0, (size_t)2 * d * f, st);
+        return e == cudaSuccess ? LB_OK : cuda_fail(e, who);
+    }
+    if (!x || !w_gate || !w_up || !w_down || !h || !kept || !dy || !workspace) return fail(LB_ERR_ARG, "%s: NULL pointer", who);
+    DeviceInfo di;
+    if ((rc = device_info(&di))) return rc;
+    const FfnPlan q = plan_ffn(n_tok, d, f, true, di.sms);
+    if (workspace_bytes < q.bytes) return fail(LB_ERR_ARG, "%s: workspace of %zu bytes, %zu are needed", who, workspace_bytes, q.bytes);
+    void *part = static_cast<char *>(workspace) + q.part;
+    char *dg = static_cast<char *>(workspace), *du = dg + (size_t)f * 2;          // [n_tok][2 f]: dg | du
+    const long long t = n_tok, f2 = 2LL * f;
+    const Operand dys[1] = {{dy, t, d, d}}, hs[1] = {{h, t, f, f}};
+    if (dx || dw_gate_up) {
+        // dh = dy Wd, turned into dg and du as it leaves the accumulators
+        const Operand wds[1] = {{w_down, d, f, f}}, outs[2] = {{dg, t, f, f2}, {du, t, f, f2}};
+        if ((rc = run_gemm(who, lb::kEpiGateBwd, lb::kFormKN, q.dh, dys, wds, outs, const_cast<void *>(kept), nullptr, t, f, d, 1, 0,
+                           di, st))) return rc;
+    }
+    if (dx) {
+        const Operand as[2] = {{dg, t, f, f2}, {du, t, f, f2}}, bs[2] = {{w_gate, f, d, d}, {w_up, f, d, d}};
+        const Operand cs[2] = {{dx, t, d, d}, {}};
+        if ((rc = run_gemm(who, lb::kEpiStore, lb::kFormKN, q.dx, as, bs, cs, nullptr, part, t, d, f, 2, 0, di, st))) return rc;
+    }
+    if (dw_gate_up) {
+        const Operand as[1] = {{dg, t, f2, f2}}, bs[1] = {{x, t, d, d}}, cs[2] = {{dw_gate_up, f2, d, d}, {}};
+        if ((rc = run_gemm(who, lb::kEpiStore, lb::kFormMN, q.dw_gu, as, bs, cs, nullptr, part, f2, d, t, 1, 0, di, st))) return rc;
+    }
+    if (dw_down) {
+        const Operand cs[2] = {{dw_down, d, f, f}, {}};
+        if ((rc = run_gemm(who, lb::kEpiStore, lb::kFormMN, q.dw_down, dys, hs, cs, nullptr, part, d, f, t, 1, 0, di, st))) return rc;
+    }
+    return LB_OK;
 }
 
 }  // extern "C"

@@ -29,6 +29,7 @@ enum DeviceError : int {
     kDevWaitScalarSlot = 4,
     kDevWaitDrain = 5,     // the producer gave up waiting for its own copies in flight at exit
     kDevWaitPeer = 6,      // the peer all-reduce gave up waiting for another rank's flag
+    kDevWaitTmem = 7,      // a matrix product gave up waiting for an accumulator
 };
 
 // The error word itself is a __device__ int owned by lb_api.cu (one per device); kernels get its address.

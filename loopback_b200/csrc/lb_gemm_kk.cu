@@ -1,0 +1,25 @@
+// Instantiations of the matrix-product kernel with A and B K-major (x W^T): the projections.
+#include "lb_gemm.cuh"
+
+namespace lb {
+
+template <int CG, int BN>
+static cudaError_t pick(int epilogue, const GemmMaps &maps, const GemmParams &p, int sms, cudaStream_t stream) {
+    switch (epilogue) {
+        case kEpiStore: return launch_gemm_t<CG, BN, kEpiStore, false, false>(maps, p, sms, stream);
+        case kEpiPartial: return launch_gemm_t<CG, BN, kEpiPartial, false, false>(maps, p, sms, stream);
+        case kEpiGate: return launch_gemm_t<CG, BN, kEpiGate, false, false>(maps, p, sms, stream);
+    }
+    return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_gemm_kk(int tile, int epilogue, const GemmMaps &maps, const GemmParams &p, int sms, cudaStream_t stream) {
+    switch (tile) {
+        case 0: return pick<1, 128>(epilogue, maps, p, sms, stream);
+        case 1: return pick<1, 256>(epilogue, maps, p, sms, stream);
+        case 2: return pick<2, 256>(epilogue, maps, p, sms, stream);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace lb

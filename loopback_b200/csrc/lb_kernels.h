@@ -8,6 +8,8 @@
 
 #define LB_DTYPE_F32 0
 #define LB_DTYPE_BF16 1
+#define LB_ACT_SILU 0
+#define LB_ACT_GELU 1
 
 namespace lb {
 
@@ -216,5 +218,46 @@ struct BlockParams {
 int block_bwd_rows(int sms);                       // CTAs of the backward at most = rows of `part`
 cudaError_t launch_block(int dtype, int wdtype, bool residual, bool bwd, const BlockParams &p, int sms, cudaStream_t stream);
 cudaError_t launch_dropout(int dtype, const void *x, void *out, long long n, const DropParams &dp, int sms, cudaStream_t stream);
+
+// The matrix products of the gated feed-forward block (lb_gemm.cuh, lb_ffn.cu)
+enum GemmEpilogue : int {
+    kEpiStore = 0,      // C rounded to bf16
+    kEpiPartial = 1,    // C in fp32 into slice `split` of a workspace (k is split; gemm_sum_kernel adds the slices in order)
+    kEpiGate = 2,       // B's tile holds two projections (g | u): h = act(g) u; act'(g) u and act(g) kept for the backward
+    kEpiGateBwd = 3,    // C = dh: dg = dh act'(g) u, du = dh act(g) from what was kept
+};
+
+struct GemmMaps {
+    CUtensorMap a[2], b[2];   // operands, one pair per segment of k (kEpiGate: b[0], b[1] are the two projections)
+    CUtensorMap c[2];         // results: boxes of 64 bf16 (32 fp32) columns x 32 rows
+};
+
+struct GemmParams {
+    int m, n;                 // rows and columns of the result (kEpiGate: columns of one projection)
+    int kblocks;              // blocks of 64 along k in one segment
+    int segs;                 // segments of k, each with operands of its own (1 or 2)
+    int m_tiles, n_tiles, splits;
+    int act;                  // LB_ACT_*
+    uint8_t *kept;            // act'(g) u and act(g) in blocks of 32 x 32 (kEpiGate: null = not kept)
+    int *err_word;
+    long long wait_cycles;
+};
+
+// operand layouts: who has k contiguous in memory
+enum GemmForm : int {
+    kFormKK = 0,        // A and B K-major:  x W^T
+    kFormKN = 1,        // A K-major, B with n contiguous:  dy W
+    kFormMN = 2,        // A with m contiguous, B with n contiguous:  dy^T x
+};
+// tile shapes the kernel is built for
+struct GemmTile {
+    int cg, bn;
+};
+constexpr GemmTile kGemmTiles[] = {{1, 128}, {1, 256}, {2, 256}};
+constexpr int kGemmTileCount = 3;
+
+cudaError_t launch_gemm(int tile, int epilogue, int form, const GemmMaps &maps, const GemmParams &p, int sms, cudaStream_t stream);
+// out[i] = sum over s of part[s][i], rounded; n a multiple of 8
+cudaError_t launch_gemm_sum(const float *part, void *out, int splits, long long n, int sms, cudaStream_t stream);
 
 }  // namespace lb

@@ -97,3 +97,58 @@ def check(name, got, want, magnitude, steps=64):
     off = (got.double() - want).abs()
     bad = ~(off <= tol)
     assert not bad.any(), f"{name}: {int(bad.sum())} of {bad.numel()} outside, worst {float((off / tol).max()):.3g} tolerances"
+
+
+def ffn(x, wg, wu, wd, act, dy=None):
+    """float64; each result with (a bound on) how far the kernels' roundings can move it: bf16 roundings of what is kept
+    between the products (h, dg, du: 2^-8 relative each; act'(g) u and act(g): cut to 24 bits, 2^-16), and fp32 accumulation, at most one rounding of
+    2^-23 (the tensor core may cut off) for every 16 columns of k, relative to the sum of the magnitudes."""
+    half, step = 2.0 ** -8, 2.0 ** -23
+    acc = lambda k: (k / 16 + 4) * step  # noqa: E731
+    d, f, t = x.shape[1], wg.shape[0], x.shape[0]
+    g, u = x @ wg.T, x @ wu.T
+    eg, eu = acc(d) * (x.abs() @ wg.abs().T), acc(d) * (x.abs() @ wu.abs().T)
+    if act == "silu":
+        s = torch.sigmoid(g)
+        a, slope = g * s, s * (1 + g * (1 - s))
+        most, curve = 1.1, 0.5                            # of |act'|, |act''|
+    else:
+        cdf, pdf = 0.5 * (1 + torch.erf(g / 2 ** 0.5)), torch.exp(-g * g / 2) / (2 * np.pi) ** 0.5
+        a, slope = g * cdf, cdf + g * pdf
+        most, curve = 1.13, 0.8
+    tiny = 16 * 2.0 ** -23                                # exp, erf and the products around them
+    h = a * u
+    eh = (1 + half) * (most * eg * u.abs() + (a.abs() + most * eg) * eu) + (half + tiny) * h.abs()
+    y = h @ wd.T
+    got = {"y": (y, eh @ wd.abs().T + acc(f) * (h.abs() @ wd.abs().T))}
+    if dy is None:
+        return got
+    dh = dy @ wd
+    edh = acc(d) * (dy.abs() @ wd.abs())
+    dg, du = dh * u * slope, dh * a
+    cut = 2.0 ** -16 + tiny
+    ep = u.abs() * curve * eg + (slope.abs() + curve * eg) * eu + cut * (u * slope).abs()      # of act'(g) u as it is kept
+    ea = most * eg + cut * a.abs()
+    edg = (1 + half) * (edh * ((u * slope).abs() + ep) + dh.abs() * ep) + half * dg.abs()
+    edu = (1 + half) * (edh * (a.abs() + ea) + dh.abs() * ea) + half * du.abs()
+    got["dx"] = dg @ wg + du @ wu, edg @ wg.abs() + edu @ wu.abs() + acc(2 * f) * (dg.abs() @ wg.abs() + du.abs() @ wu.abs())
+    got["dw_gate"] = dg.T @ x, edg.T @ x.abs() + acc(t) * (dg.abs().T @ x.abs())
+    got["dw_up"] = du.T @ x, edu.T @ x.abs() + acc(t) * (du.abs().T @ x.abs())
+    got["dw_down"] = dy.T @ h, dy.abs().T @ eh + acc(t) * (dy.abs().T @ h.abs())
+    return got
+
+
+# independent bf16 roundings on the way to each result, for the norm of its error: h or dg, du, and its own
+ROUNDINGS = 2
+
+
+def check_ffn(name, got, want, bound):
+    """Element by element against the bound (plus the result's own rounding), and, over many elements, in norm: a rounding
+    is off by at most 2^-8 relative, 2^-8 / sqrt 3 in the mean square, and independent ones add up in squares; the factor
+    sqrt 3 that is left is margin."""
+    off = (got.double() - want).abs()
+    tol = bound + 2.0 ** -8 * (want.abs() + bound) + 1e-30
+    assert bool((off <= tol).all()), f"{name}: worst {float((off / tol).max()):.3g} of its bound"
+    if want.numel() >= 4096:
+        rel = float(off.norm() / want.norm())
+        assert rel <= 2.0 ** -8 * ROUNDINGS ** 0.5, f"{name}: {rel:.3g} in norm"
