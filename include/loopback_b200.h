@@ -63,7 +63,8 @@ int lb_device_error(int clear);
  * "write_mt" (16-token tiles per consumer warp of the tensor-core write kernel: 1 or 2),
  * "write_tile" (tokens per tile of the tensor-core write kernel: a multiple of 32 up to 256), "write_stages" (its TMA
  * ring depth, 2..8), "fwd_sps" (sources per TMA stage of the forward read: 1, 2 or 4), "ffn_tile" (tile shape of the feed-forward products, 1..: an
- * index into the shapes they are built for), "ffn_splits" (slices along k, where a product may be split), "wait_cycles" (the limit of
+ * index into the shapes they are built for), "ffn_splits" (slices along k, where a product may be split), "block_frags" (16-byte fragments of a row per lane of the
+ * norm and residual kernels at most: 1..4), "wait_cycles" (the limit of
  * every bounded wait inside the kernels, in GPU clock cycles; default 4e9), "test_skip_item" (test hook: the first
  * CTA of the next forward reads leaves out its k-th tile copy, so that a bounded wait runs out, the CTA unwinds and
  * lb_device_error reports it; nothing traps or hangs). Value 0 restores the default

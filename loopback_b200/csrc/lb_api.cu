@@ -38,7 +38,7 @@ int cuda_fail(cudaError_t e, const char *what) {
 struct Options {
     int fwd_stages = 0, bwd_stages = 0, fwd_fr = 0, grid_cap = 0, fwd_warps = 0, bwd_warps = 0, bwd_wpt = 0,
         tma_per_chunk = 0, write_tt = 0, write_mt = 0, fwd_sps = 0, write_tile = 0, write_stages = 0, wait_cycles = 0, test_skip_item = 0,
-        ffn_tile = 0, ffn_splits = 0;
+        ffn_tile = 0, ffn_splits = 0, block_frags = 0;
 } g_opt;
 
 struct DeviceInfo {
@@ -214,6 +214,7 @@ int lb_set_option(const char *name, int value) {
     else if (!strcmp(name, "wait_cycles")) g_opt.wait_cycles = value;
     else if (!strcmp(name, "ffn_tile")) g_opt.ffn_tile = value;
     else if (!strcmp(name, "ffn_splits")) g_opt.ffn_splits = value;
+    else if (!strcmp(name, "block_frags")) g_opt.block_frags = value;
     else if (!strcmp(name, "test_skip_item")) g_opt.test_skip_item = value;
     else return fail(LB_ERR_ARG, "unknown option '%s'", name);
     return LB_OK;
@@ -714,6 +715,9 @@ static int check_drop(const char *who, int threshold, const int64_t *rng, const 
     return LB_OK;
 }
 
+// the "block_frags" knob: 1..4, else chosen by size
+static int block_frags() { return g_opt.block_frags >= 1 && g_opt.block_frags <= 4 ? g_opt.block_frags : 0; }
+
 static lb::DropParams drop_params(int threshold, const int64_t *rng, int64_t seed, int64_t offset, int64_t *rng_used) {
     lb::DropParams dp;
     dp.threshold = (unsigned)threshold;
@@ -769,7 +773,7 @@ int lb_norm_fwd(const void *x, const void *w, void *u, float *r, int64_t n_tok, 
     if ((rc = device_info(&di))) return rc;
     lb::BlockParams p;
     p.x = x; p.w_next = w; p.u = u; p.r_o = r; p.n_tok = n_tok; p.d = d; p.eps = eps;
-    p.frags = d / (dtype == LB_DTYPE_BF16 ? 8 : 4);
+    p.frags = d / (dtype == LB_DTYPE_BF16 ? 8 : 4); p.most_frags = block_frags();
     const cudaError_t e = lb::launch_block(dtype, wdtype, false, false, p, di.sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? LB_OK : cuda_fail(e, "lb_norm_fwd launch");
 }
@@ -783,7 +787,7 @@ int lb_norm_bwd(const void *x, const void *w, const float *r, const void *du, vo
         return fail(LB_ERR_ALIGN, "lb_norm_bwd: x, w, du and dx must be 16-byte aligned");
     lb::BlockParams p;
     p.x = x; p.w_next = w; p.r_o = const_cast<float *>(r); p.d_u = du; p.dx = dx; p.dw_next = dw; p.n_tok = n_tok; p.d = d;
-    p.frags = d / (dtype == LB_DTYPE_BF16 ? 8 : 4);
+    p.frags = d / (dtype == LB_DTYPE_BF16 ? 8 : 4); p.most_frags = block_frags();
     return finish_block_bwd("lb_norm_bwd", p, scratch, dtype, wdtype, false, static_cast<cudaStream_t>(stream));
 }
 
@@ -811,7 +815,7 @@ int lb_residual_fwd(const void *x, const void *y, const void *w, const void *gat
     p.x = x; p.y = y; p.w = w; p.gate = gate; p.gate_kind = gate_kind; p.scale_dev = scale_dev; p.scale = scale; p.w_next = next_w;
     p.out = out; p.u = u; p.r_y = r_y; p.r_o = r_o; p.n_tok = n_tok; p.d = d; p.eps = eps;
     p.drop = drop_params(threshold, rng, seed, offset, rng_used);
-    p.frags = d / (dtype == LB_DTYPE_BF16 ? 8 : 4);
+    p.frags = d / (dtype == LB_DTYPE_BF16 ? 8 : 4); p.most_frags = block_frags();
     const cudaError_t e = lb::launch_block(dtype, wdtype, true, false, p, di.sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? LB_OK : cuda_fail(e, "lb_residual_fwd launch");
 }
@@ -838,7 +842,7 @@ int lb_residual_bwd(const void *x, const void *y, const void *w, const void *gat
     p.r_y = const_cast<float *>(r_y); p.r_o = const_cast<float *>(r_o); p.d_out = d_out; p.d_u = d_u;
     p.dx = dx; p.dy = dy; p.dw = dw; p.dgate = dgate; p.dscale = dscale; p.dw_next = dnext_w; p.n_tok = n_tok; p.d = d;
     p.drop = drop_params(threshold, rng, seed, offset, nullptr);
-    p.frags = d / (dtype == LB_DTYPE_BF16 ? 8 : 4);
+    p.frags = d / (dtype == LB_DTYPE_BF16 ? 8 : 4); p.most_frags = block_frags();
     if (!d_u) p.dw_next = nullptr;
     rc = finish_block_bwd("lb_residual_bwd", p, scratch, dtype, wdtype, true, static_cast<cudaStream_t>(stream));
     if (rc || d_u || !dnext_w) return rc;

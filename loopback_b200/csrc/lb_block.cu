@@ -12,9 +12,10 @@
 // The backward recomputes o from x and y (both have to be read for dx and dy anyway), so neither o nor the mask is saved:
 // only the two fp32 scales of each row. It reads and writes each row once.
 //
-// A row is handled by `wpt` warps (1, 2, 4 or 8 of the CTA's 8); a lane keeps FR fragments of 16 bytes of every row in
-// registers, so the row is read once although its statistics are needed before its result. All arithmetic is fp32 with one
-// rounding at each store.
+// A row is handled by `wpt` warps (1, 2, 4 or 8 of the CTA's 8); a lane owns FR fragments of 16 bytes of every row, so the row
+// is read once although its statistics are needed before its result. The rows to come are on their way into shared memory
+// (cp.async, two rows ahead, each lane fetching the fragments it will read itself: no barrier); per-channel parameters lie
+// there as fp32. All arithmetic is fp32, in pairs (fma.rn.f32x2), with one rounding at each store.
 #include "lb_common.cuh"
 #include "lb_kernels.h"
 
@@ -44,18 +45,26 @@ __device__ __forceinline__ uint4 philox4x32_10(unsigned long long group, unsigne
     return make_uint4(c0, c1, c2, c3);
 }
 
-// keeps or clears the VEC elements that start at linear index `e` (a multiple of VEC); a dropped element becomes 0 whatever
-// it held
-template <int VEC>
-__device__ __forceinline__ void drop_fragment(float (&v)[VEC], unsigned long long e, const DropParams &dp,
-                                              unsigned long long seed, unsigned long long offset) {
+// The words that decide over the fragment at linear index `e` (a multiple of 2 P), one per pair of elements
+template <int P>
+__device__ __forceinline__ void drop_words(uint32_t (&w)[P], unsigned long long e, unsigned long long seed, unsigned long long offset) {
     const uint4 q = philox4x32_10(e >> 3, offset, seed);
-    const bool high = VEC == 4 && (e & 4) != 0;
-    const uint32_t w[4] = {high ? q.z : q.x, high ? q.w : q.y, q.z, q.w};
+    if constexpr (P == 4) {
+        w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+    } else {
+        const bool high = (e & 4) != 0;
+        w[0] = high ? q.z : q.x; w[1] = high ? q.w : q.y;
+    }
+}
+// clears what is dropped, whatever it held; the factor of what stays is applied elsewhere. The upper half is at least t
+// where the word is at least t << 16, the lower one where the word shifted up is.
+template <int P>
+__device__ __forceinline__ void drop_pairs(float2 (&v)[P], const uint32_t (&w)[P], uint32_t threshold) {
+    const uint32_t t = threshold << 16;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        const uint32_t h = (j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu;
-        v[j] = h >= dp.threshold ? v[j] * dp.keep_scale : 0.f;
+    for (int i = 0; i < P; ++i) {
+        v[i].x = (w[i] << 16) >= t ? v[i].x : 0.f;
+        v[i].y = w[i] >= t ? v[i].y : 0.f;
     }
 }
 
@@ -64,15 +73,30 @@ __device__ __forceinline__ void drop_state(const DropParams &dp, unsigned long l
     offset = dp.rng ? (unsigned long long)dp.rng[1] : (unsigned long long)dp.offset;
 }
 
-// VEC weights (storage type W) from column c on
+__device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Per-channel parameters in shared memory, fp32, in planes of 4 columns per fragment (a lane reads 16 bytes of each plane:
+// no bank conflicts). dst[plane][frag][4] = a[c] * b[c], 1 where a pointer is null.
 template <typename W, int VEC>
-__device__ __forceinline__ void load_weights(const W *p, long long c, float (&f)[VEC]) {
-    if constexpr (Store<W>::kVec == VEC) {
-        Store<W>::unpack(*reinterpret_cast<const uint4 *>(p + c), f);
-    } else {                                            // bf16 rows, fp32 weights
-        const float4 a = *reinterpret_cast<const float4 *>(p + c), b = *reinterpret_cast<const float4 *>(p + c + 4);
-        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-        f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+__device__ __forceinline__ void stage_channels(float *dst, const W *a, const W *b, int d, int frags) {
+    for (int c = threadIdx.x; c < d; c += kBlkThreads) {
+        const float v = (a ? Store<W>::load1(a + c) : 1.f) * (b ? Store<W>::load1(b + c) : 1.f);
+        dst[(((c % VEC) >> 2) * frags + c / VEC) * 4 + (c & 3)] = v;
+    }
+}
+template <int P>
+__device__ __forceinline__ void channel_pairs(float2 (&v)[P], uint32_t base, uint32_t plane) {
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) {
+        const float4 q = lds_f4(base + i * plane);
+        v[2 * i] = make_float2(q.x, q.y);
+        v[2 * i + 1] = make_float2(q.z, q.w);
     }
 }
 
@@ -90,17 +114,58 @@ __device__ __forceinline__ float row_sum(float v, int wpt, int grp, int wl, int 
     return t;
 }
 
+// Shared memory of both kernels: the ring [array][2 rows ahead][FR][thread] of 16 bytes, then the two channel tables; the
+// backward's column sums take the ring's place at the end.
+constexpr int kSlot = kBlkThreads * 16;
+__host__ __device__ constexpr int ring_bytes(int arrays, int fr) { return 2 * arrays * fr * kSlot; }
+
 template <typename T, typename W, int FR, bool RES>
 __global__ void __launch_bounds__(kBlkThreads) block_fwd_kernel(const BlockParams p) {
     using S = Store<T>;
-    constexpr int VEC = S::kVec;
+    constexpr int VEC = S::kVec, P = S::kPairs;
     __shared__ float slots[2][kBlkWarps];
+    extern __shared__ __align__(16) uint8_t dyn[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int wpt = p.wpt, groups = kBlkWarps / wpt, grp = warp / wpt, wl = warp % wpt;
     const T *x = static_cast<const T *>(p.x), *y = static_cast<const T *>(p.y);
+    const T *gate = p.gate_kind == kGateFull ? static_cast<const T *>(p.gate) : nullptr;
     const W *w = static_cast<const W *>(p.w), *w2 = static_cast<const W *>(p.w_next);
     T *out = static_cast<T *>(p.out), *u = static_cast<T *>(p.u);
-    const float s = RES ? (p.scale_dev ? *p.scale_dev : p.scale) : 0.f;
+    const int arrays = RES ? (gate ? 3 : 2) : 1;
+    const int f0 = wl * FR * 32 + lane;                  // this lane's fragments: f0, f0 + 32, ..
+    const long long own = (long long)f0 * VEC;
+    const uint32_t ring = smem_u32(dyn) + threadIdx.x * 16;
+    float *tab = reinterpret_cast<float *>(dyn + ring_bytes(arrays, FR));
+    const uint32_t tab_wg = smem_u32(tab) + f0 * 16, tab_w2 = tab_wg + (RES ? p.frags * VEC * 4 : 0), plane = p.frags * 16;
+    const auto slot = [&](int stage, int array, int k) { return ring + stage * (FR * kSlot) + (array * 2 * FR + k) * kSlot; };
+    const auto fetch = [&](int stage, long long tok) {
+        if (tok < p.n_tok) {
+            const long long row = tok * p.d + own;           // this lane's first element of the row
+#pragma unroll
+            for (int k = 0; k < FR; ++k) {
+                const int f = f0 + 32 * k;
+                if (f < p.frags) {
+                    cp_async16(slot(stage, 0, k), x + row + k * 32 * VEC);
+                    if constexpr (RES) {
+                        cp_async16(slot(stage, 1, k), y + row + k * 32 * VEC);
+                        if (gate) cp_async16(slot(stage, 2, k), gate + row + k * 32 * VEC);
+                    }
+                }
+            }
+        }
+        cp_async_commit();
+    };
+    const long long step = (long long)gridDim.x * groups;
+    long long tok = (long long)blockIdx.x * groups + grp;
+    fetch(0, tok);
+    fetch(1, tok + step);
+    if constexpr (RES) {
+        stage_channels<W, VEC>(tab, w, p.gate_kind == kGateChannel ? static_cast<const W *>(p.gate) : nullptr, p.d, p.frags);
+        if (w2) stage_channels<W, VEC>(tab + p.frags * VEC, w2, nullptr, p.d, p.frags);
+    } else {
+        stage_channels<W, VEC>(tab, w2, nullptr, p.d, p.frags);
+    }
+    const float s = RES ? (p.scale_dev ? *p.scale_dev : p.scale) * p.drop.keep_scale : 0.f;
     const float inv_d = 1.f / (float)p.d;
     unsigned long long seed = 0, offset = 0;
     if (RES && p.drop.threshold) {
@@ -110,81 +175,86 @@ __global__ void __launch_bounds__(kBlkThreads) block_fwd_kernel(const BlockParam
             p.drop.rng_used[1] = (long long)offset;
         }
     }
-    int turn = 0;
-    const long long step = (long long)gridDim.x * groups;
-    for (long long tok = (long long)blockIdx.x * groups + grp; tok < p.n_tok; tok += step) {
-        const long long row = tok * p.d;
-        uint4 xq[FR], yq[RES ? FR : 1];
-#pragma unroll
-        for (int k = 0; k < FR; ++k) {
-            const int f = (k * wpt + wl) * 32 + lane;
-            const bool in = f < p.frags;
-            xq[k] = in ? ld_global_stream_v4(x + row + f * VEC) : make_uint4(0, 0, 0, 0);
-            if constexpr (RES) yq[k] = in ? ld_global_stream_v4(y + row + f * VEC) : make_uint4(0, 0, 0, 0);
-        }
-        float o[FR][VEC];
+    __syncthreads();
+    int turn = 0, stage = 0;
+    for (; tok < p.n_tok; tok += step, stage ^= 1) {
+        const long long row = tok * p.d + own;           // this lane's first element of the row
+        cp_async_wait<1>();
+        float2 o[FR][P];
         if constexpr (RES) {
+            uint4 yq[FR];
             float ry = 1.f;
+#pragma unroll
+            for (int k = 0; k < FR; ++k) {
+                const bool in = f0 + 32 * k < p.frags;
+                yq[k] = in ? lds_v4(slot(stage, 1, k)) : make_uint4(0, 0, 0, 0);
+            }
             if (w) {
-                float ss = 0.f;
+                float2 ss = splat(0.f);
 #pragma unroll
                 for (int k = 0; k < FR; ++k) {
-                    float v[VEC];
-                    S::unpack(yq[k], v);
+                    float2 v[P];
+                    S::unpack2(yq[k], v);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) ss = fmaf(v[e], v[e], ss);
+                    for (int i = 0; i < P; ++i) ss = __ffma2_rn(v[i], v[i], ss);
                 }
-                ry = rsqrtf(row_sum(ss, wpt, grp, wl, lane, slots, turn) * inv_d + p.eps);
+                ry = rsqrtf(row_sum(ss.x + ss.y, wpt, grp, wl, lane, slots, turn) * inv_d + p.eps);
                 if (p.r_y && wl == 0 && lane == 0) p.r_y[tok] = ry;
             }
             const float gt = p.gate_kind == kGateToken ? S::load1(static_cast<const T *>(p.gate) + tok) : 1.f;
-            const float sg = s * gt;
+            const float2 sg = splat(s * gt), ry2 = splat(ry);
 #pragma unroll
             for (int k = 0; k < FR; ++k) {
-                const int f = (k * wpt + wl) * 32 + lane;
-                const bool in = f < p.frags;
-                float b[VEC], g[VEC];
-                S::unpack(yq[k], b);
-                S::unpack(xq[k], o[k]);
-                if (in) {
-                    if (w) {
-                        load_weights<W, VEC>(w, f * VEC, g);
+                const int f = f0 + 32 * k;
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) b[e] = g[e] * (b[e] * ry);
+                for (int i = 0; i < P; ++i) o[k][i] = splat(0.f);
+                if (f < p.frags) {
+                    float2 b[P], c[P];
+                    S::unpack2(yq[k], b);
+                    channel_pairs<P>(c, tab_wg + k * 512, plane);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) b[i] = __fmul2_rn(c[i], __fmul2_rn(b[i], ry2));
+                    if (gate) {
+                        S::unpack2(lds_v4(slot(stage, 2, k)), c);
+#pragma unroll
+                        for (int i = 0; i < P; ++i) b[i] = __fmul2_rn(b[i], c[i]);
                     }
-                    if (p.drop.threshold) drop_fragment<VEC>(b, (unsigned long long)(row + f * VEC), p.drop, seed, offset);
-                    if (p.gate_kind == kGateChannel) load_weights<W, VEC>(static_cast<const W *>(p.gate), f * VEC, g);
-                    else if (p.gate_kind == kGateFull) S::unpack(ld_global_stream_v4(static_cast<const T *>(p.gate) + row + f * VEC), g);
-                    if (p.gate_kind >= kGateChannel) {
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) b[e] *= g[e];
+                    if (p.drop.threshold) {
+                        uint32_t words[P];
+                        drop_words<P>(words, (unsigned long long)(row + k * 32 * VEC), seed, offset);
+                        drop_pairs<P>(b, words, p.drop.threshold);
                     }
+                    S::unpack2(lds_v4(slot(stage, 0, k)), o[k]);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) o[k][e] = fmaf(sg, b[e], o[k][e]);
-                    st_global_v4(out + row + f * VEC, S::pack(o[k]));
+                    for (int i = 0; i < P; ++i) o[k][i] = __ffma2_rn(sg, b[i], o[k][i]);
+                    st_global_v4(out + row + k * 32 * VEC, S::pack2v(o[k]));
                 }
             }
-            if (!w2) continue;
         } else {
 #pragma unroll
-            for (int k = 0; k < FR; ++k) S::unpack(xq[k], o[k]);
+            for (int k = 0; k < FR; ++k) {
+                const bool in = f0 + 32 * k < p.frags;
+                S::unpack2(in ? lds_v4(slot(stage, 0, k)) : make_uint4(0, 0, 0, 0), o[k]);
+            }
         }
-        float ss = 0.f;
+        fetch(stage, tok + 2 * step);
+        if (RES && !w2) continue;
+        float2 ss = splat(0.f);
 #pragma unroll
         for (int k = 0; k < FR; ++k)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) ss = fmaf(o[k][e], o[k][e], ss);
-        const float ro = rsqrtf(row_sum(ss, wpt, grp, wl, lane, slots, turn) * inv_d + p.eps);
+            for (int i = 0; i < P; ++i) ss = __ffma2_rn(o[k][i], o[k][i], ss);
+        const float ro = rsqrtf(row_sum(ss.x + ss.y, wpt, grp, wl, lane, slots, turn) * inv_d + p.eps);
         if (p.r_o && wl == 0 && lane == 0) p.r_o[tok] = ro;
 #pragma unroll
         for (int k = 0; k < FR; ++k) {
-            const int f = (k * wpt + wl) * 32 + lane;
+            const int f = f0 + 32 * k;
             if (f < p.frags) {
-                float g[VEC];
-                load_weights<W, VEC>(w2, f * VEC, g);
+                float2 c[P];
+                channel_pairs<P>(c, tab_w2 + k * 512, plane);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) g[e] *= o[k][e] * ro;
-                st_global_v4(u + row + f * VEC, S::pack(g));
+                for (int i = 0; i < P; ++i) c[i] = __fmul2_rn(c[i], __fmul2_rn(o[k][i], splat(ro)));
+                st_global_v4(u + row + k * 32 * VEC, S::pack2v(c));
             }
         }
     }
@@ -192,194 +262,210 @@ __global__ void __launch_bounds__(kBlkThreads) block_fwd_kernel(const BlockParam
 
 // Per-CTA column sums leave through p.part[CTA][2][d] (A, then B); block_param_kernel adds the CTAs' rows in a fixed order.
 template <typename T, typename W, int FR, bool RES>
-__global__ void __launch_bounds__(kBlkThreads) block_bwd_kernel(const BlockParams p) {
+__global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && sizeof(T) == 4) ? 2 : 1) block_bwd_kernel(const BlockParams p) {
     using S = Store<T>;
-    constexpr int VEC = S::kVec;
+    constexpr int VEC = S::kVec, P = S::kPairs;
     __shared__ float slots[2][kBlkWarps];
-    extern __shared__ float cols[];                      // [2][d], only when several rows share the CTA
+    extern __shared__ __align__(16) uint8_t dyn[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int wpt = p.wpt, groups = kBlkWarps / wpt, grp = warp / wpt, wl = warp % wpt;
     const T *x = static_cast<const T *>(p.x), *y = static_cast<const T *>(p.y);
     const T *dout = static_cast<const T *>(p.d_out), *du = static_cast<const T *>(p.d_u);
+    const T *gate = p.gate_kind == kGateFull ? static_cast<const T *>(p.gate) : nullptr;
     const W *w = static_cast<const W *>(p.w), *w2 = static_cast<const W *>(p.w_next);
     T *dx = static_cast<T *>(p.dx), *dy = static_cast<T *>(p.dy);
-    const float s = RES ? (p.scale_dev ? *p.scale_dev : p.scale) : 0.f;
+    // arrays of the ring: du, x, then y, dout, gate
+    const int arrays = RES ? (gate ? 5 : 4) : 2;
+    const int f0 = wl * FR * 32 + lane;                  // this lane's fragments: f0, f0 + 32, ..
+    const long long own = (long long)f0 * VEC;
+    const uint32_t ring = smem_u32(dyn) + threadIdx.x * 16;
+    float *tab = reinterpret_cast<float *>(dyn + ring_bytes(arrays, FR));
+    const uint32_t tab_wg = smem_u32(tab) + f0 * 16, tab_w2 = tab_wg + (RES ? p.frags * VEC * 4 : 0), plane = p.frags * 16;
+    const auto slot = [&](int stage, int array, int k) { return ring + stage * (FR * kSlot) + (array * 2 * FR + k) * kSlot; };
+    const auto fetch = [&](int stage, long long tok) {
+        if (tok < p.n_tok) {
+            const long long row = tok * p.d + own;           // this lane's first element of the row
+#pragma unroll
+            for (int k = 0; k < FR; ++k) {
+                const int f = f0 + 32 * k;
+                if (f < p.frags) {
+                    if (du) {
+                        cp_async16(slot(stage, 0, k), du + row + k * 32 * VEC);
+                        cp_async16(slot(stage, 1, k), x + row + k * 32 * VEC);
+                    }
+                    if constexpr (RES) {
+                        cp_async16(slot(stage, 2, k), y + row + k * 32 * VEC);
+                        if (dout) cp_async16(slot(stage, 3, k), dout + row + k * 32 * VEC);
+                        if (gate) cp_async16(slot(stage, 4, k), gate + row + k * 32 * VEC);
+                    }
+                }
+            }
+        }
+        cp_async_commit();
+    };
+    const long long step = (long long)gridDim.x * groups;
+    long long tok = (long long)blockIdx.x * groups + grp;
+    fetch(0, tok);
+    fetch(1, tok + step);
+    if constexpr (RES) {
+        stage_channels<W, VEC>(tab, w, p.gate_kind == kGateChannel ? static_cast<const W *>(p.gate) : nullptr, p.d, p.frags);
+        if (du) stage_channels<W, VEC>(tab + p.frags * VEC, w2, nullptr, p.d, p.frags);
+    } else {
+        stage_channels<W, VEC>(tab, w2, nullptr, p.d, p.frags);
+    }
+    const float s = RES ? (p.scale_dev ? *p.scale_dev : p.scale) * p.drop.keep_scale : 0.f;
     const float inv_d = 1.f / (float)p.d;
     unsigned long long seed = 0, offset = 0;
     if (RES && p.drop.threshold) drop_state(p.drop, seed, offset);
     if (blockIdx.x == 0 && threadIdx.x == 0 && p.counter) *p.counter = 0;    // block_param_kernel counts its CTAs here
-    float colA[RES ? FR : 1][VEC], colB[FR][VEC];
+    float2 colA[RES ? FR : 1][P], colB[FR][P];
 #pragma unroll
     for (int k = 0; k < FR; ++k)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            colB[k][e] = 0.f;
-            if constexpr (RES) colA[k][e] = 0.f;
+        for (int i = 0; i < P; ++i) {
+            colB[k][i] = splat(0.f);
+            if constexpr (RES) colA[k][i] = splat(0.f);
         }
-    int turn = 0;
-    const long long step = (long long)gridDim.x * groups;
-    for (long long tok = (long long)blockIdx.x * groups + grp; tok < p.n_tok; tok += step) {
-        const long long row = tok * p.d;
+    __syncthreads();
+    int turn = 0, stage = 0;
+    for (; tok < p.n_tok; tok += step, stage ^= 1) {
+        const long long row = tok * p.d + own;           // this lane's first element of the row
         const float ry = RES && w ? p.r_y[tok] : 1.f;
         const float ro = du ? p.r_o[tok] : 0.f;
         const float gt = RES && p.gate_kind == kGateToken ? S::load1(static_cast<const T *>(p.gate) + tok) : 1.f;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        uint4 xq[FR], uq[FR], yq[RES ? FR : 1], gq[RES ? FR : 1];
-        float D[FR][VEC];
-#pragma unroll
-        for (int k = 0; k < FR; ++k) {
-            const int f = (k * wpt + wl) * 32 + lane;
-            const bool in = f < p.frags;
-            uq[k] = in && du ? ld_global_stream_v4(du + row + f * VEC) : zero;
-            xq[k] = in && du ? ld_global_stream_v4(x + row + f * VEC) : zero;
-            if constexpr (RES) {
-                yq[k] = in ? ld_global_stream_v4(y + row + f * VEC) : zero;
-                gq[k] = in && dout ? ld_global_stream_v4(dout + row + f * VEC) : zero;
-            }
-        }
+        const float2 ry2 = splat(ry), ro2 = splat(ro);
+        cp_async_wait<1>();
+        float2 D[FR][P], oh[FR][P], yh[RES ? FR : 1][P];
+        uint32_t words[RES ? FR : 1][P];
+        float2 acc = splat(0.f);
         // the gradient of o through its norm
-        float oh[FR][VEC];
-        float acc = 0.f;
 #pragma unroll
         for (int k = 0; k < FR; ++k) {
-            const int f = (k * wpt + wl) * 32 + lane;
+            const int f = f0 + 32 * k;
+            const bool in = f < p.frags;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) D[k][e] = oh[k][e] = 0.f;
-            if (f < p.frags && du) {
-                float g[VEC];
-                S::unpack(xq[k], oh[k]);
+            for (int i = 0; i < P; ++i) D[k][i] = oh[k][i] = splat(0.f);
+            if constexpr (RES) {
+                S::unpack2(in ? lds_v4(slot(stage, 2, k)) : make_uint4(0, 0, 0, 0), yh[k]);
+#pragma unroll
+                for (int i = 0; i < P; ++i) yh[k][i] = __fmul2_rn(yh[k][i], ry2);
+                if (in && p.drop.threshold) drop_words<P>(words[k], (unsigned long long)(row + k * 32 * VEC), seed, offset);
+            }
+            if (in && du) {
+                float2 c[P];
+                S::unpack2(lds_v4(slot(stage, 1, k)), oh[k]);
                 if constexpr (RES) {
-                    float b[VEC];
-                    S::unpack(yq[k], b);
-                    if (w) {
-                        load_weights<W, VEC>(w, f * VEC, g);
+                    float2 b[P];
+                    channel_pairs<P>(c, tab_wg + k * 512, plane);
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) b[e] = g[e] * (b[e] * ry);
+                    for (int i = 0; i < P; ++i) b[i] = __fmul2_rn(c[i], yh[k][i]);
+                    if (gate) {
+                        S::unpack2(lds_v4(slot(stage, 4, k)), c);
+#pragma unroll
+                        for (int i = 0; i < P; ++i) b[i] = __fmul2_rn(b[i], c[i]);
                     }
-                    if (p.drop.threshold) drop_fragment<VEC>(b, (unsigned long long)(row + f * VEC), p.drop, seed, offset);
-                    if (p.gate_kind == kGateChannel) load_weights<W, VEC>(static_cast<const W *>(p.gate), f * VEC, g);
-                    else if (p.gate_kind == kGateFull) S::unpack(ld_global_stream_v4(static_cast<const T *>(p.gate) + row + f * VEC), g);
-                    if (p.gate_kind >= kGateChannel) {
+                    if (p.drop.threshold) drop_pairs<P>(b, words[k], p.drop.threshold);
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) b[e] *= g[e];
-                    }
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) oh[k][e] = fmaf(s * gt, b[e], oh[k][e]);
+                    for (int i = 0; i < P; ++i) oh[k][i] = __ffma2_rn(splat(s * gt), b[i], oh[k][i]);
                 }
-                float uu[VEC];
-                S::unpack(uq[k], uu);
-                load_weights<W, VEC>(w2, f * VEC, g);
+                float2 uu[P];
+                S::unpack2(lds_v4(slot(stage, 0, k)), uu);
+                channel_pairs<P>(c, tab_w2 + k * 512, plane);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    oh[k][e] *= ro;
-                    colB[k][e] = fmaf(uu[e], oh[k][e], colB[k][e]);
-                    D[k][e] = g[e] * uu[e];
-                    acc = fmaf(D[k][e], oh[k][e], acc);
+                for (int i = 0; i < P; ++i) {
+                    oh[k][i] = __fmul2_rn(oh[k][i], ro2);
+                    colB[k][i] = __ffma2_rn(uu[i], oh[k][i], colB[k][i]);
+                    D[k][i] = __fmul2_rn(c[i], uu[i]);
+                    acc = __ffma2_rn(D[k][i], oh[k][i], acc);
                 }
             }
         }
         if (du) {
-            const float c1 = row_sum(acc, wpt, grp, wl, lane, slots, turn) * inv_d;
+            const float2 c1 = splat(-row_sum(acc.x + acc.y, wpt, grp, wl, lane, slots, turn) * inv_d);
 #pragma unroll
             for (int k = 0; k < FR; ++k)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) D[k][e] = ro * fmaf(-c1, oh[k][e], D[k][e]);
+                for (int i = 0; i < P; ++i) D[k][i] = __fmul2_rn(ro2, __ffma2_rn(c1, oh[k][i], D[k][i]));
         }
         if constexpr (!RES) {
+            fetch(stage, tok + 2 * step);
 #pragma unroll
             for (int k = 0; k < FR; ++k) {
-                const int f = (k * wpt + wl) * 32 + lane;
-                if (f < p.frags && dx) st_global_v4(dx + row + f * VEC, S::pack(D[k]));
+                const int f = f0 + 32 * k;
+                if (f < p.frags && dx) st_global_v4(dx + row + k * 32 * VEC, S::pack2v(D[k]));
             }
         } else {
-            float S1 = 0.f;                              // sum of w g (m D) yh: the token gate's gradient and the norm's mean
+            float2 sum = splat(0.f);                     // of w g (m D) yh: the token gate's gradient and the norm's mean
 #pragma unroll
             for (int k = 0; k < FR; ++k) {
-                const int f = (k * wpt + wl) * 32 + lane;
+                const int f = f0 + 32 * k;
                 if (f >= p.frags) continue;
-                float v[VEC];
-                S::unpack(gq[k], v);
+                if (dout) {
+                    float2 v[P];
+                    S::unpack2(lds_v4(slot(stage, 3, k)), v);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) D[k][e] += v[e];
-                if (dx) st_global_v4(dx + row + f * VEC, S::pack(D[k]));
-                if (p.drop.threshold) drop_fragment<VEC>(D[k], (unsigned long long)(row + f * VEC), p.drop, seed, offset);
-                float yh[VEC], g[VEC];
-                S::unpack(yq[k], yh);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) yh[e] *= ry;
-                if (p.gate_kind == kGateChannel) {
-                    load_weights<W, VEC>(static_cast<const W *>(p.gate), f * VEC, g);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        colA[k][e] = fmaf(D[k][e], yh[e], colA[k][e]);
-                        D[k][e] *= g[e];
-                    }
-                } else if (p.gate_kind == kGateFull) {
-                    float dg[VEC];
-                    if (w) load_weights<W, VEC>(w, f * VEC, dg);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) dg[e] = s * ((w ? dg[e] : 1.f) * (D[k][e] * yh[e]));
-                    if (p.dgate) st_global_v4(static_cast<T *>(p.dgate) + row + f * VEC, S::pack(dg));
-                    S::unpack(ld_global_stream_v4(static_cast<const T *>(p.gate) + row + f * VEC), g);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        D[k][e] *= g[e];
-                        colA[k][e] = fmaf(D[k][e], yh[e], colA[k][e]);
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) colA[k][e] = fmaf(gt * D[k][e], yh[e], colA[k][e]);
+                    for (int i = 0; i < P; ++i) D[k][i] = __fadd2_rn(D[k][i], v[i]);
                 }
-                if (w) {
-                    load_weights<W, VEC>(w, f * VEC, g);
+                if (dx) st_global_v4(dx + row + k * 32 * VEC, S::pack2v(D[k]));
+                if (p.drop.threshold) drop_pairs<P>(D[k], words[k], p.drop.threshold);
+                float2 c[P];
+                channel_pairs<P>(c, tab_wg + k * 512, plane);
+                if (gate) {
+                    float2 g[P];
+                    if (p.dgate) {
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) D[k][e] *= g[e];
+                        for (int i = 0; i < P; ++i) g[i] = __fmul2_rn(splat(s), __fmul2_rn(c[i], __fmul2_rn(D[k][i], yh[k][i])));
+                        st_global_v4(static_cast<T *>(p.dgate) + row + k * 32 * VEC, S::pack2v(g));
+                    }
+                    S::unpack2(lds_v4(slot(stage, 4, k)), g);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) D[k][i] = __fmul2_rn(D[k][i], g[i]);
                 }
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) S1 = fmaf(D[k][e], yh[e], S1);
+                for (int i = 0; i < P; ++i) {
+                    const float2 a = p.gate_kind == kGateToken ? __fmul2_rn(splat(gt), D[k][i]) : D[k][i];
+                    colA[k][i] = __ffma2_rn(a, yh[k][i], colA[k][i]);
+                    D[k][i] = __fmul2_rn(D[k][i], c[i]);
+                    sum = __ffma2_rn(D[k][i], yh[k][i], sum);
+                }
             }
+            fetch(stage, tok + 2 * step);
+            float S1 = sum.x + sum.y;
             if (w || p.gate_kind == kGateToken) S1 = row_sum(S1, wpt, grp, wl, lane, slots, turn);
             if (p.gate_kind == kGateToken && p.dgate && wl == 0 && lane == 0) S::store1(static_cast<T *>(p.dgate) + tok, s * S1);
             if (dy) {
-                const float sg = s * gt, c2 = w ? S1 * inv_d : 0.f;
+                const float2 k1 = splat(s * gt * ry), c2 = splat(w ? -S1 * inv_d : 0.f);
 #pragma unroll
                 for (int k = 0; k < FR; ++k) {
-                    const int f = (k * wpt + wl) * 32 + lane;
+                    const int f = f0 + 32 * k;
                     if (f >= p.frags) continue;
-                    float yh[VEC];
-                    S::unpack(yq[k], yh);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) D[k][e] = sg * (ry * fmaf(-c2, yh[e] * ry, D[k][e]));
-                    st_global_v4(dy + row + f * VEC, S::pack(D[k]));
+                    for (int i = 0; i < P; ++i) D[k][i] = __fmul2_rn(k1, __ffma2_rn(c2, yh[k][i], D[k][i]));
+                    st_global_v4(dy + row + k * 32 * VEC, S::pack2v(D[k]));
                 }
             }
         }
     }
     if (!p.part) return;
     float *mine = p.part + (long long)blockIdx.x * 2 * p.d;
-    if (groups == 1) {
-#pragma unroll
-        for (int k = 0; k < FR; ++k) {
-            const int f = (k * wpt + wl) * 32 + lane;
-            if (f >= p.frags) continue;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                if constexpr (RES) mine[f * VEC + e] = colA[k][e];
-                mine[p.d + f * VEC + e] = colB[k][e];
-            }
-        }
-        return;
-    }
+    float *cols = reinterpret_cast<float *>(dyn);        // [2][d]
+    cp_async_wait<0>();
+    __syncthreads();
     for (int g = 0; g < groups; ++g) {                   // the CTA's rows in order: the sums do not depend on timing
         if (grp == g) {
 #pragma unroll
             for (int k = 0; k < FR; ++k) {
-                const int f = (k * wpt + wl) * 32 + lane;
+                const int f = f0 + 32 * k;
                 if (f >= p.frags) continue;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    if constexpr (RES) cols[f * VEC + e] = (g ? cols[f * VEC + e] : 0.f) + colA[k][e];
-                    cols[p.d + f * VEC + e] = (g ? cols[p.d + f * VEC + e] : 0.f) + colB[k][e];
+                for (int i = 0; i < P; ++i) {
+                    const int c = f * VEC + 2 * i;
+                    if constexpr (RES) {
+                        cols[c] = (g ? cols[c] : 0.f) + colA[k][i].x;
+                        cols[c + 1] = (g ? cols[c + 1] : 0.f) + colA[k][i].y;
+                    }
+                    cols[p.d + c] = (g ? cols[p.d + c] : 0.f) + colB[k][i].x;
+                    cols[p.d + c + 1] = (g ? cols[p.d + c + 1] : 0.f) + colB[k][i].y;
                 }
             }
         }
@@ -391,39 +477,48 @@ __global__ void __launch_bounds__(kBlkThreads) block_bwd_kernel(const BlockParam
     }
 }
 
-// Column sums over the CTAs' rows, in fp64, and the parameters' gradients from them. 32 columns per CTA, 8 row strides.
+// Column sums over the CTAs' rows, in fp64, and the parameters' gradients from them. 32 columns per CTA, 32 row strides.
 // The residual scale's gradient needs all columns: the CTA that comes last adds the others' parts, in order.
 template <typename W>
-__global__ void __launch_bounds__(kBlkThreads) block_param_kernel(const BlockParams p, int rows) {
-    __shared__ double sa[8][33], sb[8][33];
-    __shared__ bool last;
+__global__ void __launch_bounds__(1024) block_param_kernel(const BlockParams p, int rows) {
+    __shared__ double sa[32][33], sb[32][33];
     const int c = threadIdx.x & 31, r0 = threadIdx.x >> 5;
     const int col = blockIdx.x * 32 + c;
     double a = 0., b = 0.;
     if (col < p.d) {
-        for (int r = r0; r < rows; r += 8) {
-            const float *q = p.part + (long long)r * 2 * p.d;
-            if (p.need_a) a += q[col];
-            if (p.dw_next) b += q[p.d + col];
+        const float *q = p.part + (long long)r0 * 2 * p.d + col;
+        for (int r = r0; r < rows; r += 128, q += 256LL * p.d) {             // four rows in flight
+            float va[4], vb[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool in = r + 32 * i < rows;
+                va[i] = in && p.need_a ? q[64LL * i * p.d] : 0.f;
+                vb[i] = in && p.dw_next ? q[64LL * i * p.d + p.d] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                a += va[i];
+                b += vb[i];
+            }
         }
     }
     sa[r0][c] = a;
     sb[r0][c] = b;
     __syncthreads();
     if (r0 == 0) {
-        for (int i = 1; i < 8; ++i) {
+        for (int i = 1; i < 32; ++i) {
             a += sa[i][c];
             b += sb[i][c];
         }
         double ds = 0.;
         if (col < p.d) {
-            const float s = p.scale_dev ? *p.scale_dev : p.scale;
+            const float s = (p.scale_dev ? *p.scale_dev : p.scale) * p.drop.keep_scale;
             const float w = p.w ? Store<W>::load1(static_cast<const W *>(p.w) + col) : 1.f;
             const float g = p.gate_kind == kGateChannel ? Store<W>::load1(static_cast<const W *>(p.gate) + col) : 1.f;
             if (p.dw) Store<W>::store1(static_cast<W *>(p.dw) + col, (float)(a * s * g));
             if (p.dgate && p.gate_kind == kGateChannel) Store<W>::store1(static_cast<W *>(p.dgate) + col, (float)(a * s * w));
             if (p.dw_next) Store<W>::store1(static_cast<W *>(p.dw_next) + col, (float)b);
-            ds = a * w * g;
+            ds = a * w * g * p.drop.keep_scale;
         }
         if (p.dscale) {
             for (int o = 16; o > 0; o >>= 1) ds += __shfl_xor_sync(0xffffffffu, ds, o);
@@ -433,8 +528,7 @@ __global__ void __launch_bounds__(kBlkThreads) block_param_kernel(const BlockPar
     if (!p.dscale) return;
     if (threadIdx.x == 0) {
         __threadfence();
-        last = atomicAdd(p.counter, 1u) == gridDim.x - 1;
-        if (last) {
+        if (atomicAdd(p.counter, 1u) == gridDim.x - 1) {
             __threadfence();
             double t = 0.;
             for (unsigned i = 0; i < gridDim.x; ++i) t += *reinterpret_cast<volatile double *>(p.ds_part + i);
@@ -454,20 +548,35 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T *__restrict__ x, T
         dp.rng_used[0] = (long long)seed;
         dp.rng_used[1] = (long long)offset;
     }
+    constexpr int P = S::kPairs;
     const long long frags = n / VEC, stride = (long long)gridDim.x * blockDim.x;
+    const float2 scale = splat(dp.keep_scale);
+    const auto masked = [&](const uint4 &q, long long f) {
+        float2 v[P];
+        uint32_t words[P];
+        S::unpack2(q, v);
+        drop_words<P>(words, (unsigned long long)(f * VEC), seed, offset);
+#pragma unroll
+        for (int i = 0; i < P; ++i) v[i] = __fmul2_rn(v[i], scale);
+        drop_pairs<P>(v, words, dp.threshold);
+        return S::pack2v(v);
+    };
     long long f = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    for (; f < frags; f += stride) {
-        float v[VEC];
-        S::unpack(ld_global_stream_v4(x + f * VEC), v);
-        drop_fragment<VEC>(v, (unsigned long long)(f * VEC), dp, seed, offset);
-        st_global_v4(out + f * VEC, S::pack(v));
+    for (; f + 3 * stride < frags; f += 4 * stride) {    // four fragments in flight
+        uint4 q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = ld_global_stream_v4(x + (f + i * stride) * VEC);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st_global_v4(out + (f + i * stride) * VEC, masked(q[i], f + i * stride));
     }
+    for (; f < frags; f += stride) st_global_v4(out + f * VEC, masked(ld_global_stream_v4(x + f * VEC), f));
     if (f == frags && frags * VEC < n) {                 // the elements behind the last whole fragment: one thread
-        float v[VEC];
-        for (int e = 0; e < VEC; ++e) v[e] = frags * VEC + e < n ? S::load1(x + frags * VEC + e) : 0.f;
-        drop_fragment<VEC>(v, (unsigned long long)(frags * VEC), dp, seed, offset);
-        for (int e = 0; e < VEC; ++e)
-            if (frags * VEC + e < n) S::store1(out + frags * VEC + e, v[e]);
+        uint32_t words[P];
+        drop_words<P>(words, (unsigned long long)(frags * VEC), seed, offset);
+        for (int e = 0; frags * VEC + e < n; ++e) {
+            const uint32_t h = e & 1 ? words[e >> 1] >> 16 : words[e >> 1] & 0xffffu;
+            S::store1(out + frags * VEC + e, h >= dp.threshold ? S::load1(x + frags * VEC + e) * dp.keep_scale : 0.f);
+        }
     }
 }
 
@@ -487,33 +596,54 @@ static bool block_shape(int frags, long long n_tok, int sms, int most, int *fr, 
     return need <= 4;
 }
 
+// CTAs of 256 threads an SM holds, by registers (of 65,536, in units of 256 per warp) and shared memory
+static int registers_of(const void *kernel) {
+    cudaFuncAttributes at;
+    if (cudaFuncGetAttributes(&at, kernel) == cudaSuccess) return at.numRegs;
+    cudaGetLastError();
+    return 255;
+}
+static int resident(int regs, size_t smem) {
+    const int by_regs = 65536 / (kBlkWarps * ((regs * 32 + 255) / 256 * 256));
+    const int by_smem = (int)((size_t)(228 * 1024) / (smem + 64 + 1024));
+    const int n = by_regs < by_smem ? by_regs : by_smem;
+    return n < 1 ? 1 : n > 8 ? 8 : n;
+}
+
 template <typename T, typename W, bool RES>
 static cudaError_t launch_block_t(BlockParams p, bool bwd, int sms, cudaStream_t stream) {
     int fr;
-    if (!block_shape(p.frags, p.n_tok, sms, 4, &fr, &p.wpt)) return cudaErrorInvalidValue;
+    const int most = p.most_frags ? p.most_frags : 4;
+    if (!block_shape(p.frags, p.n_tok, sms, most, &fr, &p.wpt)) return cudaErrorInvalidValue;
     const int groups = kBlkWarps / p.wpt;
+    const bool full = p.gate_kind == kGateFull;
+    const int arrays = bwd ? (RES ? 4 + full : 2) : (RES ? 2 + full : 1);
+    size_t smem = ring_bytes(arrays, fr) + sizeof(float) * (RES ? 2 : 1) * p.frags * Store<T>::kVec;
+    if (bwd && smem < sizeof(float) * 2 * p.d) smem = sizeof(float) * 2 * p.d;
     const long long need = (p.n_tok + groups - 1) / groups;
-    const long long cap = bwd ? block_bwd_rows(sms) : 8LL * sms;
-    const int grid = (int)(need < cap ? need : cap);
-    const size_t smem = bwd && groups > 1 ? sizeof(float) * 2 * p.d : 0;
 #define LB_BLK(FR_)                                                                                                  \
-    case FR_:                                                                                                        \
-        if (bwd) {                                                                                                   \
-            if (smem > 48 * 1024) {                                                                                  \
-                const cudaError_t e = cudaFuncSetAttribute(block_bwd_kernel<T, W, FR_, RES>,                         \
-                                                           cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  \
-                if (e != cudaSuccess) return e;                                                                      \
-            }                                                                                                        \
-            block_bwd_kernel<T, W, FR_, RES><<<grid, kBlkThreads, smem, stream>>>(p);                                \
-        } else block_fwd_kernel<T, W, FR_, RES><<<grid, kBlkThreads, 0, stream>>>(p);                                \
-        break;
+    case FR_: {                                                                                                      \
+        auto kernel = bwd ? block_bwd_kernel<T, W, FR_, RES> : block_fwd_kernel<T, W, FR_, RES>;                     \
+        cudaError_t e = cudaSuccess;                                                                                 \
+        if (smem > 40 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
+        if (e != cudaSuccess) return e;                                                                              \
+        static const int regs[2] = {registers_of(reinterpret_cast<const void *>(block_fwd_kernel<T, W, FR_, RES>)),  \
+                                    registers_of(reinterpret_cast<const void *>(block_bwd_kernel<T, W, FR_, RES>))}; \
+        const int per_sm = resident(regs[bwd], smem);                                                                \
+        long long cap = (long long)sms * per_sm;                                                                     \
+        if (bwd && cap > block_bwd_rows(sms)) cap = block_bwd_rows(sms);                                             \
+        grid = (int)(need < cap ? need : cap);                                                                       \
+        kernel<<<grid, kBlkThreads, smem, stream>>>(p);                                                              \
+        break;                                                                                                       \
+    }
+    int grid = 0;
     switch (fr) {
         LB_BLK(1) LB_BLK(2) LB_BLK(3) LB_BLK(4)
     }
 #undef LB_BLK
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || !bwd || !p.part) return e;
-    block_param_kernel<W><<<(p.d + 31) / 32, kBlkThreads, 0, stream>>>(p, grid);
+    block_param_kernel<W><<<(p.d + 31) / 32, 1024, 0, stream>>>(p, grid);
     return cudaGetLastError();
 }
 

@@ -214,6 +214,7 @@ struct BlockParams {
     int d = 0, frags = 0, wpt = 1;
     int need_a = 0;                                // dw, a channel gate's gradient or dscale is wanted
     float eps = 0.f;
+    int most_frags = 0;                            // fragments per lane at most; 0 = chosen by size
 };
 int block_bwd_rows(int sms);                       // CTAs of the backward at most = rows of `part`
 cudaError_t launch_block(int dtype, int wdtype, bool residual, bool bwd, const BlockParams &p, int sms, cudaStream_t stream);
