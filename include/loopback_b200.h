@@ -63,7 +63,8 @@ int lb_device_error(int clear);
  * "write_mt" (16-token tiles per consumer warp of the tensor-core write kernel: 1 or 2),
  * "write_tile" (tokens per tile of the tensor-core write kernel: a multiple of 32 up to 256), "write_stages" (its TMA
  * ring depth, 2..8), "fwd_sps" (sources per TMA stage of the forward read: 1, 2 or 4), "ffn_tile" (tile shape of the feed-forward products, 1..: an
- * index into the shapes they are built for), "ffn_splits" (slices along k, where a product may be split), "block_frags" (16-byte fragments of a row per lane of the
+ * index into the shapes they are built for), "ffn_splits" (slices along k, where a product may be split), "ffn_small" (rows up to which a forward without
+ * gradients takes the kernels for few rows; -1 never), "block_frags" (16-byte fragments of a row per lane of the
  * norm and residual kernels at most: 1..4), "wait_cycles" (the limit of
  * every bounded wait inside the kernels, in GPU clock cycles; default 4e9), "test_skip_item" (test hook: the first
  * CTA of the next forward reads leaves out its k-th tile copy, so that a bounded wait runs out, the CTA unwinds and
@@ -314,6 +315,7 @@ int lb_dropout(const void *x, void *out, int threshold, const int64_t *rng, int6
 
 #define LB_FFN_FORWARD 0
 #define LB_FFN_BACKWARD 1
+#define LB_FFN_INFERENCE 2 /* a forward without h */
 
 /* Bytes of `workspace` a call of this size needs on the current device (0 and an error message for sizes it refuses). */
 size_t lb_ffn_workspace_bytes(int64_t n_tok, int d, int f, int kind);
@@ -322,7 +324,8 @@ size_t lb_ffn_workspace_bytes(int64_t n_tok, int d, int f, int kind);
  * act(g) with 24 bits each, 6 bytes per element of h, rows and columns rounded up to 32). */
 size_t lb_ffn_kept_bytes(int64_t n_tok, int f);
 
-/* h [n_tok][f] is written in any case (the backward wants it); kept may be NULL: no backward. */
+/* Training: h [n_tok][f] and kept are written for the backward. Inference: both NULL, and up to 128 rows (a decode step) take
+ * kernels of their own, bound by reading the weights once. */
 int lb_ffn_fwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, void *y, void *h, void *kept,
                void *workspace, size_t workspace_bytes, int64_t n_tok, int d, int f, int act, int dtype, void *stream);
 

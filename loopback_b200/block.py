@@ -284,7 +284,7 @@ def block_residual(x: torch.Tensor, y: torch.Tensor, weight=None, *, gate=None, 
 # the gated feed-forward product
 # --------------------------------------------------------------------------------------------------------------
 _ACTS = {"silu": 0, "gelu": 1}
-_FFN_FORWARD, _FFN_BACKWARD = 0, 1
+_FFN_FORWARD, _FFN_BACKWARD, _FFN_INFERENCE = 0, 1, 2
 
 
 def _ffn_workspace(n_tok, d, f, kind, dev):
@@ -298,11 +298,11 @@ def _ffn_forward(x, wg, wu, wd, act, save):
     d, f, dev = x.shape[-1], wg.shape[0], x.device
     n_tok = x.numel() // d
     y = torch.empty_like(x)
-    h = torch.empty((n_tok, f), dtype=x.dtype, device=dev)
+    h = torch.empty((n_tok, f), dtype=x.dtype, device=dev) if save else None
     with _on(dev):
-        ws = _ffn_workspace(n_tok, d, f, _FFN_FORWARD, dev)
+        ws = _ffn_workspace(n_tok, d, f, _FFN_FORWARD if save else _FFN_INFERENCE, dev)
         kept = torch.empty(int(_lib.lib().lb_ffn_kept_bytes(n_tok, f)), dtype=torch.uint8, device=dev) if save else None
-        check(_lib.lib().lb_ffn_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), h.data_ptr(), _p(kept),
+        check(_lib.lib().lb_ffn_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), _p(h), _p(kept),
                                     ws.data_ptr(), ws.numel(), n_tok, d, f, act, dtype_code(x.dtype), stream_ptr()), "gated ffn")
     return y, h, kept
 

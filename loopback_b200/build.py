@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(HERE, "libloopback_b200.so")
 SOURCES = ("lb_api.cu", "lb_write.cu", "lb_write_mma.cu", "lb_read_fwd.cu", "lb_read_bwd.cu", "lb_read_bwd_f32.cu", "lb_step.cu",
-           "lb_noalloc.cu", "lb_peer.cu", "lb_block.cu", "lb_ffn.cu",
+           "lb_noalloc.cu", "lb_peer.cu", "lb_block.cu", "lb_ffn.cu", "lb_ffn_small.cu",
            "lb_gemm_kk.cu", "lb_gemm_kn.cu", "lb_gemm_mn.cu")
 HEADERS = ("lb_common.cuh", "lb_kernels.h", "lb_read_bwd_impl.cuh", "lb_gemm.cuh", os.path.join("..", "..", "include", "loopback_b200.h"))
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -38,7 +38,7 @@ int cuda_fail(cudaError_t e, const char *what) {
 struct Options {
     int fwd_stages = 0, bwd_stages = 0, fwd_fr = 0, grid_cap = 0, fwd_warps = 0, bwd_warps = 0, bwd_wpt = 0,
         tma_per_chunk = 0, write_tt = 0, write_mt = 0, fwd_sps = 0, write_tile = 0, write_stages = 0, wait_cycles = 0, test_skip_item = 0,
-        ffn_tile = 0, ffn_splits = 0, block_frags = 0;
+        ffn_tile = 0, ffn_splits = 0, block_frags = 0, ffn_small = 0;
 } g_opt;
 
 struct DeviceInfo {
@@ -214,6 +214,7 @@ int lb_set_option(const char *name, int value) {
     else if (!strcmp(name, "wait_cycles")) g_opt.wait_cycles = value;
     else if (!strcmp(name, "ffn_tile")) g_opt.ffn_tile = value;
     else if (!strcmp(name, "ffn_splits")) g_opt.ffn_splits = value;
+    else if (!strcmp(name, "ffn_small")) g_opt.ffn_small = value;
     else if (!strcmp(name, "block_frags")) g_opt.block_frags = value;
     else if (!strcmp(name, "test_skip_item")) g_opt.test_skip_item = value;
     else return fail(LB_ERR_ARG, "unknown option '%s'", name);
@@ -961,11 +962,22 @@ static int run_gemm(const char *who, int epi, int form, const GemmPlan &pl, cons
 
 struct FfnPlan {
     GemmPlan up, down, dh, dx, dw_gu, dw_down;
-    size_t part = 0, bytes = 0;                         // offset of the slices in the workspace (dg | du lie before them), its size
+    size_t part = 0, bytes = 0;                         // offset of the slices in the workspace (dg | du, or h, lie before them), its size
 };
 
-static FfnPlan plan_ffn(long long t, long long d, long long f, bool bwd, int sms) {
+// few rows and nothing kept: the kernels of lb_ffn_small.cu. The "ffn_small" knob: rows up to which they are taken (-1: never).
+static bool ffn_small(long long t, int kind) {
+    const int most = g_opt.ffn_small < 0 ? 0 : g_opt.ffn_small > 0 && g_opt.ffn_small < lb::kFfnSmallTokens ? g_opt.ffn_small : lb::kFfnSmallTokens;
+    return kind == LB_FFN_INFERENCE && t <= most;
+}
+
+static FfnPlan plan_ffn(long long t, long long d, long long f, int kind, int sms) {
     FfnPlan q;
+    const bool bwd = kind == LB_FFN_BACKWARD;
+    if (ffn_small(t, kind)) {
+        q.bytes = (size_t)t * (size_t)f * 2;
+        return q;
+    }
     const auto blocks = [](long long k) { return (k + 63) / 64; };
     size_t part = 0;
     const auto need = [&](const GemmPlan &g, long long m, long long n) {
@@ -986,7 +998,7 @@ static FfnPlan plan_ffn(long long t, long long d, long long f, bool bwd, int sms
         need(q.dw_down, d, f);
     }
     const auto align = [](size_t b) { return (b + 255) / 256 * 256; };
-    q.part = bwd ? align((size_t)t * (size_t)f * 4) : 0;
+    q.part = bwd ? align((size_t)t * (size_t)f * 4) : kind == LB_FFN_INFERENCE ? align((size_t)t * (size_t)f * 2) : 0;
     q.bytes = q.part + part;
     return q;
 }
@@ -1003,9 +1015,13 @@ static int check_ffn(const char *who, int64_t n_tok, int d, int f, int act, int 
 
 size_t lb_ffn_workspace_bytes(int64_t n_tok, int d, int f, int kind) {
     if (check_ffn("lb_ffn_workspace_bytes", n_tok, d, f, LB_ACT_SILU, LB_DTYPE_BF16)) return 0;
+    if (kind != LB_FFN_FORWARD && kind != LB_FFN_BACKWARD && kind != LB_FFN_INFERENCE) {
+        fail(LB_ERR_ARG, "lb_ffn_workspace_bytes: unknown kind %d", kind);
+        return 0;
+    }
     DeviceInfo di;
     if (device_info(&di)) return 0;
-    return plan_ffn(n_tok, d, f, kind == LB_FFN_BACKWARD, di.sms).bytes + 16;
+    return plan_ffn(n_tok, d, f, kind, di.sms).bytes + 16;
 }
 
 size_t lb_ffn_kept_bytes(int64_t n_tok, int f) {
@@ -1019,15 +1035,32 @@ int lb_ffn_fwd(const void *x, const void *w_gate, const void *w_up, const void *
     int rc = check_ffn(who, n_tok, d, f, act, dtype);
     if (rc) return rc;
     if (n_tok == 0) return LB_OK;
-    if (!x || !w_gate || !w_up || !w_down || !y || !h || !workspace) return fail(LB_ERR_ARG, "%s: NULL pointer", who);
+    if (!x || !w_gate || !w_up || !w_down || !y || !workspace || (kept && !h)) return fail(LB_ERR_ARG, "%s: NULL pointer", who);
     if (!aligned16(x) || !aligned16(w_gate) || !aligned16(w_up) || !aligned16(w_down) || !aligned16(y) || !aligned16(h) ||
         !aligned16(kept) || !aligned16(workspace))
         return fail(LB_ERR_ALIGN, "%s: every pointer must be 16-byte aligned", who);
     DeviceInfo di;
     if ((rc = device_info(&di))) return rc;
-    const FfnPlan q = plan_ffn(n_tok, d, f, false, di.sms);
+    const int kind = h ? LB_FFN_FORWARD : LB_FFN_INFERENCE;
+    const FfnPlan q = plan_ffn(n_tok, d, f, kind, di.sms);
     if (workspace_bytes < q.bytes) return fail(LB_ERR_ARG, "%s: workspace of %zu bytes, %zu are needed", who, workspace_bytes, q.bytes);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (!h) h = workspace;
+    if (ffn_small(n_tok, kind)) {
+        const int rows = lb::ffn_small_rows(n_tok);
+        CUtensorMap m0, m1, mx;
+        lb::FfnSmallParams p;
+        p.n_tok = (int)n_tok; p.act = act; p.err_word = di.err_word; p.wait_cycles = wait_limit();
+        if ((rc = make_map_tile(&m0, w_gate, f, d, d, 64)) || (rc = make_map_tile(&m1, w_up, f, d, d, 64)) ||
+            (rc = make_map_tile(&mx, x, n_tok, d, d, rows))) return rc;
+        p.out = h; p.n = f; p.kblocks = (d + 63) / 64;
+        cudaError_t e = lb::launch_ffn_small(true, rows, m0, m1, mx, p, di.sms, st);
+        if (e != cudaSuccess) return cuda_fail(e, who);
+        if ((rc = make_map_tile(&m0, w_down, d, f, f, 128)) || (rc = make_map_tile(&mx, h, n_tok, f, f, rows))) return rc;
+        p.out = y; p.n = d; p.kblocks = (f + 63) / 64;
+        e = lb::launch_ffn_small(false, rows, m0, m0, mx, p, di.sms, st);
+        return e == cudaSuccess ? LB_OK : cuda_fail(e, who);
+    }
     void *part = static_cast<char *>(workspace) + q.part;
     const Operand xs[1] = {{x, n_tok, d, d}}, w2[2] = {{w_gate, f, d, d}, {w_up, f, d, d}}, hs[2] = {{h, n_tok, f, f}, {}};
     if ((rc = run_gemm(who, lb::kEpiGate, lb::kFormKK, q.up, xs, w2, hs, kept, nullptr, n_tok, f, d, 1, act, di, st))) return rc;
@@ -1054,7 +1087,7 @@ int lb_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *
     if (!x || !w_gate || !w_up || !w_down || !h || !kept || !dy || !workspace) return fail(LB_ERR_ARG, "%s: NULL pointer", who);
     DeviceInfo di;
     if ((rc = device_info(&di))) return rc;
-    const FfnPlan q = plan_ffn(n_tok, d, f, true, di.sms);
+    const FfnPlan q = plan_ffn(n_tok, d, f, LB_FFN_BACKWARD, di.sms);
     if (workspace_bytes < q.bytes) return fail(LB_ERR_ARG, "%s: workspace of %zu bytes, %zu are needed", who, workspace_bytes, q.bytes);
     void *part = static_cast<char *>(workspace) + q.part;
     char *dg = static_cast<char *>(workspace), *du = dg + (size_t)f * 2;          // [n_tok][2 f]: dg | du

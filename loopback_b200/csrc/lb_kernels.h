@@ -258,6 +258,20 @@ constexpr GemmTile kGemmTiles[] = {{1, 128}, {1, 256}, {2, 256}};
 constexpr int kGemmTileCount = 3;
 
 cudaError_t launch_gemm(int tile, int epilogue, int form, const GemmMaps &maps, const GemmParams &p, int sms, cudaStream_t stream);
+// the same block for few rows (lb_ffn_small.cu)
+constexpr int kFfnSmallTokens = 128;               // rows at most
+struct FfnSmallParams {
+    void *out;                // [n_tok][n]: h or y
+    int n_tok, n;             // n: columns of the result (= weight rows of one projection)
+    int kblocks;              // blocks of 64 along k
+    int act;
+    int split = 1, stages = 1;   // CTAs per tile, ring depth (filled in by the launcher)
+    int *err_word;
+    long long wait_cycles;
+};
+int ffn_small_rows(long long n_tok);               // tokens rounded up to what the kernel is built for
+cudaError_t launch_ffn_small(bool gated, int rows, const CUtensorMap &w0, const CUtensorMap &w1, const CUtensorMap &x,
+                             const FfnSmallParams &p, int sms, cudaStream_t stream);
 // out[i] = sum over s of part[s][i], rounded; n a multiple of 8
 cudaError_t launch_gemm_sum(const float *part, void *out, int splits, long long n, int sms, cudaStream_t stream);
 

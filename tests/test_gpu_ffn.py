@@ -72,7 +72,7 @@ def test_same_bits_every_run():
 
 
 @pytest.mark.parametrize("t", [1, 2, 15, 16, 17, 33, 64, 65, 100, 128, 129, 200])
-@pytest.mark.parametrize("d,f", [(64, 128), (768, 2048), (1000, 1416), (2048, 5632)])
+@pytest.mark.parametrize("d,f", [(8, 8), (64, 128), (136, 40), (768, 2048), (1000, 1416), (2048, 5632), (4096, 1024)])
 def test_few_rows_without_gradients(t, d, f):
     from loopback_b200 import block
     (x, wg, wu, wd), _ = _inputs(t, d, f, t + d, grad=False)
@@ -81,6 +81,9 @@ def test_few_rows_without_gradients(t, d, f):
     ref.check_ffn("y", y, *want["y"])
     with torch.no_grad():
         assert torch.equal(block.gated_ffn(x, wg, wu, wd), y)
+    if t > 1:                                             # a batch padded with rows that hold no number
+        x[-1] = float("nan")
+        assert torch.equal(block.gated_ffn(x, wg, wu, wd)[:-1], y[:-1])
 
 
 def test_rows_behind_the_last_stay():
@@ -90,12 +93,20 @@ def test_rows_behind_the_last_stay():
         (x, wg, wu, wd), _ = _inputs(t, 136, 264, 5, grad=False)
         y = torch.full((t + 40, 136), 7.0, device="cuda", dtype=torch.bfloat16)
         h = torch.full((t + 40, 264), 7.0, device="cuda", dtype=torch.bfloat16)
+        kept = torch.empty(L.lib().lb_ffn_kept_bytes(t, 264), device="cuda", dtype=torch.uint8)
         n = L.lib().lb_ffn_workspace_bytes(t, 136, 264, 0)
         ws = torch.full((n // 4 + 1,), float("nan"), device="cuda")
-        L.check(L.lib().lb_ffn_fwd(L.ptr(x), L.ptr(wg), L.ptr(wu), L.ptr(wd), L.ptr(y), L.ptr(h), None, L.ptr(ws), n, t, 136, 264, 0,
+        L.check(L.lib().lb_ffn_fwd(L.ptr(x), L.ptr(wg), L.ptr(wu), L.ptr(wd), L.ptr(y), L.ptr(h), L.ptr(kept), L.ptr(ws), n, t, 136, 264, 0,
                                    L.LB_DTYPE_BF16, L.stream_ptr()), "gated ffn")
         ref.check_ffn("y", y[:t], *ref.ffn(*(v.double() for v in (x, wg, wu, wd)), "silu")["y"])
         assert bool((y[t:] == 7).all()) and bool((h[t:] == 7).all())
+        y.fill_(7.0)
+        n = L.lib().lb_ffn_workspace_bytes(t, 136, 264, 2)
+        ws = torch.full((n // 4 + 1,), float("nan"), device="cuda")
+        L.check(L.lib().lb_ffn_fwd(L.ptr(x), L.ptr(wg), L.ptr(wu), L.ptr(wd), L.ptr(y), None, None, L.ptr(ws), n, t, 136, 264, 0,
+                                   L.LB_DTYPE_BF16, L.stream_ptr()), "gated ffn")
+        ref.check_ffn("y", y[:t], *ref.ffn(*(v.double() for v in (x, wg, wu, wd)), "silu")["y"])
+        assert bool((y[t:] == 7).all())
 
 
 def test_special_values_stay_in_their_rows():
