@@ -18,12 +18,26 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import check, dtype_code, stream_ptr
-from .fused_dattn import _on, _require_cuda
+from ._lib import check, dtype_code
+from .fused_dattn import _require_cuda
 
 __all__ = ["block_norm", "block_residual", "dropout", "gated_ffn"]
 
 GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_FULL = range(4)
+
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _call(x, what, fn, *args):
+    """fn(*args, stream) on x's device, on its current stream. A decode step is bound by what the host does per call, so this
+    avoids the guard and the Stream object where x's device is the current one."""
+    dev = x.get_device()
+    if dev == _current_device():
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    check(rc, what)
 
 
 def _p(t):
@@ -31,34 +45,35 @@ def _p(t):
 
 
 def _require_rows(x, what):
-    _require_cuda(x, what)
+    if not x.is_cuda:
+        _require_cuda(x, what)
     if x.dim() == 0 or x.shape[-1] == 0:
         raise RuntimeError(f"loopback_b200.{what}: rows need a last dimension of at least one column, got shape {tuple(x.shape)}")
 
 
 def _same_device(what, ref, *tensors):
+    dev = ref.device
     for t in tensors:
-        if t is not None and t.device != ref.device:
-            raise RuntimeError(f"loopback_b200.{what}: a tensor is on {t.device}, the rows are on {ref.device}")
-
-
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"loopback_b200.{what}: a tensor is on {t.device}, the rows are on {dev}")
 
 
 def _scratch(d, dev):
-    return torch.empty(int(_lib.lib().lb_block_scratch_bytes(d)), dtype=torch.uint8, device=dev)
+    return torch.empty(_lib.lib().lb_block_scratch_bytes(d), dtype=torch.uint8, device=dev)
 
 
 def _channel_params(what, x, d, *params):
     """The per-channel parameters in one storage type the kernels take: the rows' or, where they are fp32 or differ, fp32."""
-    types = {p.dtype for p in params if p is not None}
+    kind, cast = None, False
     for p in params:
-        if p is not None and p.shape != (d,):
-            raise RuntimeError(f"loopback_b200.{what}: a per-channel parameter has shape {tuple(p.shape)}, rows have {d} columns")
-    if len(types) > 1 or not types <= {x.dtype, torch.float32}:
-        params = tuple(p if p is None else p.float() for p in params)
-    return tuple(p if p is None else p.contiguous() for p in params)
+        if p is not None:
+            if p.shape != (d,):
+                raise RuntimeError(f"loopback_b200.{what}: a per-channel parameter has shape {tuple(p.shape)}, rows have {d} columns")
+            cast = cast or (p.dtype != kind and kind is not None) or (p.dtype != x.dtype and p.dtype != torch.float32)
+            kind = p.dtype
+    if cast:
+        params = [p if p is None else p.float() for p in params]
+    return [p if p is None else p.contiguous() for p in params]
 
 
 # --------------------------------------------------------------------------------------------------------------
@@ -69,9 +84,8 @@ def _norm_forward(x, w, eps, save):
     n_tok = x.numel() // d
     u = torch.empty_like(x)
     r = torch.empty(n_tok, dtype=torch.float32, device=x.device) if save else None
-    with _on(x.device):
-        check(_lib.lib().lb_norm_fwd(x.data_ptr(), w.data_ptr(), u.data_ptr(), _p(r), n_tok, d, eps, dtype_code(x.dtype),
-                                     dtype_code(w.dtype), stream_ptr()), "block norm")
+    _call(x, "block norm", _lib.lib().lb_norm_fwd, x.data_ptr(), w.data_ptr(), u.data_ptr(), _p(r), n_tok, d, eps,
+          dtype_code(x.dtype), dtype_code(w.dtype))
     return u, r
 
 
@@ -90,11 +104,9 @@ class _BlockNorm(torch.autograd.Function):
         du = du.contiguous()
         dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
         dw = torch.empty_like(w) if ctx.needs_input_grad[1] else None
-        with _on(x.device):
-            scratch = _scratch(d, x.device) if dw is not None else None
-            check(_lib.lib().lb_norm_bwd(x.data_ptr(), w.data_ptr(), r.data_ptr(), du.data_ptr(), _p(dx), _p(dw), _p(scratch),
-                                         x.numel() // d, d, dtype_code(x.dtype), dtype_code(w.dtype), stream_ptr()),
-                  "block norm backward")
+        scratch = _scratch(d, x.device) if dw is not None else None
+        _call(x, "block norm backward", _lib.lib().lb_norm_bwd, x.data_ptr(), w.data_ptr(), r.data_ptr(), du.data_ptr(), _p(dx),
+              _p(dw), _p(scratch), x.numel() // d, d, dtype_code(x.dtype), dtype_code(w.dtype))
         return dx, dw, None
 
 
@@ -105,7 +117,7 @@ def block_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torc
     _same_device("block_norm", x, weight)
     (w,) = _channel_params("block_norm", x, x.shape[-1], weight)
     x = x.contiguous()
-    if _wants_grad(x, w):
+    if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         return _BlockNorm.apply(x, w, float(eps))
     return _norm_forward(x, w, float(eps), False)[0]
 
@@ -136,9 +148,8 @@ def _rng_args(what, x, rng):
 
 def _dropout_launch(x, threshold, rng, seed, offset, used):
     out = torch.empty_like(x)
-    with _on(x.device):
-        check(_lib.lib().lb_dropout(x.data_ptr(), out.data_ptr(), threshold, _p(rng), seed, offset, _p(used), x.numel(),
-                                    dtype_code(x.dtype), stream_ptr()), "dropout")
+    _call(x, "dropout", _lib.lib().lb_dropout, x.data_ptr(), out.data_ptr(), threshold, _p(rng), seed, offset, _p(used), x.numel(),
+          dtype_code(x.dtype))
     return out
 
 
@@ -171,7 +182,7 @@ def dropout(x: torch.Tensor, p: float, rng) -> torch.Tensor:
     t = _threshold("dropout", p)
     pair, seed, offset = _rng_args("dropout", x, rng)
     x = x.contiguous()
-    if _wants_grad(x):
+    if x.requires_grad and torch.is_grad_enabled():
         return _Dropout.apply(x, t, pair, seed, offset)
     return _dropout_launch(x, t, pair, seed, offset, None)
 
@@ -186,7 +197,8 @@ def _wcode(x, w, gate, kind, next_w):
     return dtype_code(x.dtype)
 
 
-def _residual_forward(x, y, w, gate, scale_t, next_w, kind, scale, eps, threshold, rng, seed, offset, save):
+def _residual_forward(x, y, w, gate, scale_t, next_w, args, save):
+    kind, scale, eps, threshold, rng, seed, offset = args
     d = x.shape[-1]
     n_tok, dev = x.numel() // d, x.device
     out = torch.empty_like(x)
@@ -194,21 +206,18 @@ def _residual_forward(x, y, w, gate, scale_t, next_w, kind, scale, eps, threshol
     ry = torch.empty(n_tok, dtype=torch.float32, device=dev) if save and w is not None else None
     ro = torch.empty(n_tok, dtype=torch.float32, device=dev) if save and next_w is not None else None
     used = torch.empty_like(rng) if save and rng is not None else None
-    with _on(dev):
-        check(_lib.lib().lb_residual_fwd(x.data_ptr(), y.data_ptr(), _p(w), _p(gate), kind, _p(scale_t), scale, _p(next_w),
-                                         out.data_ptr(), _p(u), _p(ry), _p(ro), threshold, _p(rng), seed, offset, _p(used),
-                                         n_tok, d, eps, dtype_code(x.dtype), _wcode(x, w, gate, kind, next_w), stream_ptr()),
-              "block residual")
+    _call(x, "block residual", _lib.lib().lb_residual_fwd, x.data_ptr(), y.data_ptr(), _p(w), _p(gate), kind, _p(scale_t), scale,
+          _p(next_w), out.data_ptr(), _p(u), _p(ry), _p(ro), threshold, _p(rng), seed, offset, _p(used), n_tok, d, eps,
+          dtype_code(x.dtype), _wcode(x, w, gate, kind, next_w))
     return out, u, ry, ro, used
 
 
 class _BlockResidual(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, y, w, gate, scale_t, next_w, kind, scale, eps, threshold, rng, seed, offset):
-        out, u, ry, ro, used = _residual_forward(x, y, w, gate, scale_t, next_w, kind, scale, eps, threshold, rng, seed, offset,
-                                                 True)
+    def forward(ctx, x, y, w, gate, scale_t, next_w, args):
+        out, u, ry, ro, used = _residual_forward(x, y, w, gate, scale_t, next_w, args, True)
         ctx.save_for_backward(x, y, w, gate, scale_t, next_w, ry, ro, used)
-        ctx.args = kind, scale, threshold, seed, offset
+        ctx.args = args
         ctx.set_materialize_grads(False)
         return (out, u) if u is not None else out
 
@@ -216,25 +225,22 @@ class _BlockResidual(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g_out, g_u=None):
         x, y, w, gate, scale_t, next_w, ry, ro, used = ctx.saved_tensors
-        kind, scale, threshold, seed, offset = ctx.args
-        none = (None,) * 7
+        kind, scale, _, threshold, _, seed, offset = ctx.args
         if g_out is None and g_u is None:
-            return (None,) * 6 + none
+            return (None,) * 7
         d, dev = x.shape[-1], x.device
         g_out = None if g_out is None else g_out.contiguous()
         g_u = None if g_u is None else g_u.contiguous()
         grads = [torch.empty_like(t) if t is not None and need else None
                  for t, need in zip((x, y, w, gate, scale_t, next_w), ctx.needs_input_grad)]
         dx, dy, dw, dgate, dscale, dnext = grads
-        with _on(dev):
-            sums = dw is not None or dscale is not None or dnext is not None or (dgate is not None and kind == GATE_CHANNEL)
-            scratch = _scratch(d, dev) if sums else None
-            check(_lib.lib().lb_residual_bwd(x.data_ptr(), y.data_ptr(), _p(w), _p(gate), kind, _p(scale_t), scale, _p(next_w),
-                                             _p(ry), _p(ro), threshold, _p(used), seed, offset, _p(g_out), _p(g_u), _p(dx),
-                                             _p(dy), _p(dw), _p(dgate), _p(dscale), _p(dnext), _p(scratch), x.numel() // d, d,
-                                             dtype_code(x.dtype), _wcode(x, w, gate, kind, next_w), stream_ptr()),
-                  "block residual backward")
-        return (*grads, *none)
+        sums = dw is not None or dscale is not None or dnext is not None or (dgate is not None and kind == GATE_CHANNEL)
+        scratch = _scratch(d, dev) if sums else None
+        _call(x, "block residual backward", _lib.lib().lb_residual_bwd, x.data_ptr(), y.data_ptr(), _p(w), _p(gate), kind,
+              _p(scale_t), scale, _p(next_w), _p(ry), _p(ro), threshold, _p(used), seed, offset, _p(g_out), _p(g_u), _p(dx), _p(dy),
+              _p(dw), _p(dgate), _p(dscale), _p(dnext), _p(scratch), x.numel() // d, d, dtype_code(x.dtype),
+              _wcode(x, w, gate, kind, next_w))
+        return (*grads, None)
 
 
 def block_residual(x: torch.Tensor, y: torch.Tensor, weight=None, *, gate=None, scale=1.0, next_weight=None,
@@ -274,9 +280,10 @@ def block_residual(x: torch.Tensor, y: torch.Tensor, weight=None, *, gate=None, 
     t = _threshold("block_residual", p)
     pair, seed, offset = _rng_args("block_residual", x, rng) if t else (None, 0, 0)
     x, y = x.contiguous(), y.contiguous()
-    if _wants_grad(x, y, w, gate, scale_t, next_w):
-        return _BlockResidual.apply(x, y, w, gate, scale_t, next_w, kind, float(scale), float(eps), t, pair, seed, offset)
-    out, u = _residual_forward(x, y, w, gate, scale_t, next_w, kind, float(scale), float(eps), t, pair, seed, offset, False)[:2]
+    args = kind, float(scale), float(eps), t, pair, seed, offset
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, w, gate, scale_t, next_w)):
+        return _BlockResidual.apply(x, y, w, gate, scale_t, next_w, args)
+    out, u = _residual_forward(x, y, w, gate, scale_t, next_w, args, False)[:2]
     return out if u is None else (out, u)
 
 
@@ -287,23 +294,29 @@ _ACTS = {"silu": 0, "gelu": 1}
 _FFN_FORWARD, _FFN_BACKWARD, _FFN_INFERENCE = 0, 1, 2
 
 
-def _ffn_workspace(n_tok, d, f, kind, dev):
-    nbytes = int(_lib.lib().lb_ffn_workspace_bytes(n_tok, d, f, kind))
+def _ffn_workspace(x, n_tok, d, f, kind):
+    dev = x.get_device()
+    if dev == _current_device():
+        nbytes = _lib.lib().lb_ffn_workspace_bytes(n_tok, d, f, kind)
+    else:
+        with torch.cuda.device(dev):
+            nbytes = _lib.lib().lb_ffn_workspace_bytes(n_tok, d, f, kind)
     if nbytes == 0:
         raise RuntimeError("loopback_b200.gated_ffn: " + _lib.lib().lb_last_error_string().decode("utf-8", "replace"))
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return torch.empty(nbytes, dtype=torch.uint8, device=x.device), nbytes
 
 
 def _ffn_forward(x, wg, wu, wd, act, save):
-    d, f, dev = x.shape[-1], wg.shape[0], x.device
+    d, f = x.shape[-1], wg.shape[0]
     n_tok = x.numel() // d
     y = torch.empty_like(x)
-    h = torch.empty((n_tok, f), dtype=x.dtype, device=dev) if save else None
-    with _on(dev):
-        ws = _ffn_workspace(n_tok, d, f, _FFN_FORWARD if save else _FFN_INFERENCE, dev)
-        kept = torch.empty(int(_lib.lib().lb_ffn_kept_bytes(n_tok, f)), dtype=torch.uint8, device=dev) if save else None
-        check(_lib.lib().lb_ffn_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), _p(h), _p(kept),
-                                    ws.data_ptr(), ws.numel(), n_tok, d, f, act, dtype_code(x.dtype), stream_ptr()), "gated ffn")
+    h = kept = None
+    if save:
+        h = torch.empty((n_tok, f), dtype=x.dtype, device=x.device)
+        kept = torch.empty(_lib.lib().lb_ffn_kept_bytes(n_tok, f), dtype=torch.uint8, device=x.device)
+    ws, nbytes = _ffn_workspace(x, n_tok, d, f, _FFN_FORWARD if save else _FFN_INFERENCE)
+    _call(x, "gated ffn", _lib.lib().lb_ffn_fwd, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), _p(h),
+          _p(kept), ws.data_ptr(), nbytes, n_tok, d, f, act, _lib.LB_DTYPE_BF16)
     return y, h, kept
 
 
@@ -318,18 +331,17 @@ class _GatedFFN(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, wg, wu, wd, h, kept = ctx.saved_tensors
-        d, f, dev = x.shape[-1], wg.shape[0], x.device
+        d, f = x.shape[-1], wg.shape[0]
         n_tok = x.numel() // d
         dy = dy.contiguous()
         need = ctx.needs_input_grad
         dx = torch.empty_like(x) if need[0] else None
-        dgu = torch.empty((2, f, d), dtype=x.dtype, device=dev) if need[1] or need[2] else None
+        dgu = torch.empty((2, f, d), dtype=x.dtype, device=x.device) if need[1] or need[2] else None
         dwd = torch.empty_like(wd) if need[3] else None
-        with _on(dev):
-            ws = _ffn_workspace(n_tok, d, f, _FFN_BACKWARD, dev)
-            check(_lib.lib().lb_ffn_bwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), h.data_ptr(), kept.data_ptr(),
-                                        dy.data_ptr(), _p(dx), _p(dgu), _p(dwd), ws.data_ptr(), ws.numel(), n_tok, d, f,
-                                        dtype_code(x.dtype), stream_ptr()), "gated ffn backward")
+        ws, nbytes = _ffn_workspace(x, n_tok, d, f, _FFN_BACKWARD)
+        _call(x, "gated ffn backward", _lib.lib().lb_ffn_bwd, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(),
+              h.data_ptr(), kept.data_ptr(), dy.data_ptr(), _p(dx), _p(dgu), _p(dwd), ws.data_ptr(), nbytes, n_tok, d, f,
+              _lib.LB_DTYPE_BF16)
         return dx, dgu[0] if need[1] else None, dgu[1] if need[2] else None, dwd, None
 
 
@@ -348,13 +360,12 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if w_gate.dim() != 2 or w_gate.shape[1] != d or w_up.shape != w_gate.shape or w_down.shape != w_gate.shape[::-1]:
         raise RuntimeError(f"loopback_b200.gated_ffn: rows have {d} columns, weights are {tuple(w_gate.shape)}, "
                            f"{tuple(w_up.shape)}, {tuple(w_down.shape)}; expected (f, d), (f, d), (d, f)")
-    for t in (x, w_gate, w_up, w_down):
-        if t.dtype != torch.bfloat16:
-            raise RuntimeError(f"loopback_b200.gated_ffn: the products run in bf16, got {t.dtype}")
-    for t in (w_gate, w_up, w_down):
-        if not t.is_contiguous():
-            raise RuntimeError("loopback_b200.gated_ffn: weights must be contiguous")
+    if not x.dtype == w_gate.dtype == w_up.dtype == w_down.dtype == torch.bfloat16:
+        raise RuntimeError(f"loopback_b200.gated_ffn: the products run in bf16, got rows of {x.dtype} and weights of "
+                           f"{w_gate.dtype}, {w_up.dtype}, {w_down.dtype}")
+    if not (w_gate.is_contiguous() and w_up.is_contiguous() and w_down.is_contiguous()):
+        raise RuntimeError("loopback_b200.gated_ffn: weights must be contiguous")
     x = x.contiguous()
-    if _wants_grad(x, w_gate, w_up, w_down):
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
         return _GatedFFN.apply(x, w_gate, w_up, w_down, _ACTS[act])
     return _ffn_forward(x, w_gate, w_up, w_down, _ACTS[act], False)[0]
