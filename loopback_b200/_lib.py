@@ -89,6 +89,27 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_torch_ops = None
+
+
+def torch_ops():
+    """The C++ autograd nodes (csrc/lb_torch.cpp), bound to the entry points of lib(); raises if they have not been built."""
+    global _torch_ops
+    if _torch_ops is None:
+        path = os.path.join(_HERE, "_torch_ops.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: the autograd nodes of loopback_b200 are not built "
+                               "(run `python -m loopback_b200.build`); there is no fallback path")
+        from importlib.machinery import ExtensionFileLoader
+        from importlib.util import module_from_spec, spec_from_file_location
+        spec = spec_from_file_location("loopback_b200._torch_ops", path, loader=ExtensionFileLoader("loopback_b200._torch_ops", path))
+        ops = module_from_spec(spec)
+        spec.loader.exec_module(ops)
+        ops.bind({name: ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value for name in SYMBOLS})
+        _torch_ops = ops
+    return _torch_ops
+
+
 def dtype_code(dtype: torch.dtype) -> int:
     if dtype == torch.bfloat16:
         return LB_DTYPE_BF16
@@ -108,12 +129,11 @@ def stream_ptr(device=None):
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index))
 
 
-# kernels launched through this binding since import (lb_read_bwd launches two: the backward and the reduction
-# of its query-gradient partials); read by the benchmark
+# kernels launched through this binding (not through torch_ops) since import (lb_read_bwd launches two: the backward and the
+# reduction of its query-gradient partials); read by the benchmark
 LAUNCHES = {"count": 0}
 _KERNELS_PER_CALL = {"read backward": 2, "read backward (final)": 2, "combine backward": 2, "step backward": 2,
-                     "step backward (deferred)": 2, "block norm backward": 2, "block residual backward": 2,
-                     "gated ffn": 2, "gated ffn backward": 4}
+                     "step backward (deferred)": 2}
 
 
 def check(rc: int, what: str) -> None:

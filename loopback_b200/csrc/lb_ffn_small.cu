@@ -136,8 +136,13 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(const __grid_c
         if constexpr (GATED) {
             const int col = row0 + 2 * lane;
             float g0, g1, slope;
-            act_both(a[0], p.act, g0, slope);
-            act_both(a[1], p.act, g1, slope);
+            if (p.act == LB_ACT_SILU) {
+                act_both<LB_ACT_SILU>(a[0], g0, slope);
+                act_both<LB_ACT_SILU>(a[1], g1, slope);
+            } else {
+                act_both<LB_ACT_GELU>(a[0], g0, slope);
+                act_both<LB_ACT_GELU>(a[1], g1, slope);
+            }
             if (col < p.n) *reinterpret_cast<uint32_t *>(out + col) = B::pack2(g0 * a[2], g1 * a[3]);
         } else {
             const int col = row0 + 4 * lane;

@@ -157,9 +157,11 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const W
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, wc, what));
 }
 
-// act(g) and act'(g)
-__device__ __forceinline__ void act_both(float g, int act, float &a, float &slope) {
-    if (act == LB_ACT_SILU) {
+// act(g) and act'(g). The activation is a template parameter: as a run-time choice it put a branch behind every element of the
+// epilogue (106 us instead of 62 for 8192 x 1024 -> 2816).
+template <int ACT>
+__device__ __forceinline__ void act_both(float g, float &a, float &slope) {
+    if constexpr (ACT == LB_ACT_SILU) {
         const float s = __fdividef(1.f, 1.f + __expf(-g));
         a = g * s;
         slope = s * fmaf(g, 1.f - s, 1.f);
@@ -220,7 +222,7 @@ __device__ __forceinline__ TileAt tile_at(long long t, const GemmParams &p) {
     return a;
 }
 
-template <int CG, int BN, int EPI, bool A_MN, bool B_MN>
+template <int CG, int BN, int EPI, bool A_MN, bool B_MN, int ACT>
 __global__ void __launch_bounds__(GemmShape<CG, BN, EPI>::kThreads, 1)
 gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
     using Sh = GemmShape<CG, BN, EPI>;
@@ -435,7 +437,7 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
                                 float a, slope;
-                                act_both(g[8 * q + e], p.act, a, slope);
+                                act_both<ACT>(g[8 * q + e], a, slope);
                                 h[e] = a * u[8 * q + e];
                                 g[8 * q + e] = a;
                                 u[8 * q + e] *= slope;
@@ -516,10 +518,10 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
     if (warp == 1) tmem_free<CG>(tmem, Sh::kCols);
 }
 
-template <int CG, int BN, int EPI, bool A_MN, bool B_MN>
+template <int CG, int BN, int EPI, bool A_MN, bool B_MN, int ACT = 0>
 cudaError_t launch_gemm_t(const GemmMaps &maps, const GemmParams &p, int sms, cudaStream_t stream) {
     using Sh = GemmShape<CG, BN, EPI>;
-    auto kernel = gemm_kernel<CG, BN, EPI, A_MN, B_MN>;
+    auto kernel = gemm_kernel<CG, BN, EPI, A_MN, B_MN, ACT>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
     if (e != cudaSuccess) return e;
     const long long tiles = (long long)p.m_tiles * p.n_tiles * p.splits;

@@ -8,7 +8,9 @@ static cudaError_t pick(int epilogue, const GemmMaps &maps, const GemmParams &p,
     switch (epilogue) {
         case kEpiStore: return launch_gemm_t<CG, BN, kEpiStore, false, false>(maps, p, sms, stream);
         case kEpiPartial: return launch_gemm_t<CG, BN, kEpiPartial, false, false>(maps, p, sms, stream);
-        case kEpiGate: return launch_gemm_t<CG, BN, kEpiGate, false, false>(maps, p, sms, stream);
+        case kEpiGate:
+            return p.act == LB_ACT_SILU ? launch_gemm_t<CG, BN, kEpiGate, false, false, LB_ACT_SILU>(maps, p, sms, stream)
+                                        : launch_gemm_t<CG, BN, kEpiGate, false, false, LB_ACT_GELU>(maps, p, sms, stream);
     }
     return cudaErrorInvalidValue;
 }

@@ -312,3 +312,14 @@ def test_refusals():
                  lambda: block.dropout(x, float("nan"), (1, 2)), lambda: block.block_residual(x, x, p=0.5)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_second_derivatives_raise():
+    """The operators are differentiable once: under create_graph a second derivative raises instead of being taken for zero."""
+    from loopback_b200 import block
+    x = torch.randn(4, 64, device="cuda").requires_grad_()
+    w = torch.ones(64, device="cuda").requires_grad_()
+    for f in (lambda: block.block_norm(x, w), lambda: block.block_residual(x, x, w, next_weight=w)[1], lambda: block.dropout(x, 0.5, (1, 2))):
+        (g,) = torch.autograd.grad(f().square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            g.sum().backward()
