@@ -912,13 +912,15 @@ static GemmPlan plan_gemm(long long m, long long n, long long blocks, bool gate,
         const int cg = lb::kGemmTiles[i].cg, bn = lb::kGemmTiles[i].bn;
         const long long tm = 128LL * cg, tn = gate ? bn / 2 : bn, groups = sms / cg;
         const long long mt = (m + tm - 1) / tm, nt = (n + tn - 1) / tn;
-        for (int s = 1; s <= 16; ++s) {
-            if (s > 1 && (!may_split || blocks / s < 4)) break;
-            if (may_split && g_opt.ffn_splits > 0 && s != g_opt.ffn_splits) continue;
+        const int most = !may_split || blocks < 8 ? 1 : blocks / 4 < 16 ? (int)(blocks / 4) : 16;
+        const int forced = g_opt.ffn_splits <= 0 || !may_split ? 0 : g_opt.ffn_splits < most ? g_opt.ffn_splits : most;
+        for (int s = forced ? forced : 1; s <= (forced ? forced : most); ++s) {
             const double waves = (double)((mt * nt * s + groups - 1) / groups);
-            const double rate = (cg == 2 ? 1.0 : bn == 256 ? 1.15 : 1.35) * bn / 256. * 0.41;          // us per block of 64
-            double us = waves * (double)((blocks + s - 1) / s) * rate + 4.0 + bn / 128.;
-            if (s > 1) us += 3.0 + (double)s * m * n * 8. / 4.0e6;                                     // slices out and in
+            // us per block of 64 of a tile, as measured with the SMs busy (a 128 x 128 tile is bound by what L2 delivers, the
+            // 256-row one by the tensor cores), a launch's fixed part, and the slices' way out and in
+            const double rate = cg == 2 ? 0.345 : bn == 256 ? 0.39 : 0.30;
+            double us = waves * (double)((blocks + s - 1) / s) * rate + 4.5 + bn / 128. + (cg == 2 ? 1.0 : 0.0);
+            if (s > 1) us += 2.0 + (double)s * m * n * 8. / 5.0e6;
             if (us < best_us) { best_us = us; best.tile = i; best.splits = s; best.m_tiles = (int)mt; best.n_tiles = (int)nt; }
         }
     }

@@ -8,7 +8,10 @@
 //
 //   projections  tile = 64 rows of Wg over 64 rows of Wu, k over d;  epilogue h = act(g) u
 //   down         tile = 128 rows of Wd, k over f. Launched with programmatic stream serialisation: its CTAs take the SMs as
-//                the projections' leave them and have their first weights in flight before h is there.
+//                the projections' leave them and have their first weights in flight before h is there. (Measured and left out
+//                for 1 x 2048 x 5632: asking for Wd into L2 from the projections' CTAs, which made those as much longer, 19.7 us
+//                against 18.1; tiles of 64 rows of Wd, 19.3; shorter rings, so that both launches' CTAs are resident, 18.7 and
+//                31 instead of 23 at 64 rows.)
 #include "lb_gemm.cuh"
 
 namespace lb {
@@ -29,6 +32,16 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(const __grid_c
     const uint32_t rank = p.split > 1 ? cluster_rank() : 0;
     const int tile = blockIdx.x / p.split;
     WaitCtx wc{abort_flag, p.err_word, p.wait_cycles};
+    const int kb0 = (int)((long long)p.kblocks * rank / p.split), kb1 = (int)((long long)p.kblocks * (rank + 1) / p.split);
+    const int row0 = tile * (GATED ? 64 : 128);
+    const int ahead = kb1 - kb0 < ST ? kb1 - kb0 : ST;
+    const auto weights = [&](int s, int kb) {
+        const uint32_t sa = base + s * kStage, bar = full + 8 * s;
+        mbar_arrive_expect_tx(bar, kStage);
+        tma_load_2d(sa, &map_w0, bar, kb * kGemmK, row0);
+        if constexpr (GATED) tma_load_2d(sa + kA / 2, &map_w1, bar, kb * kGemmK, row0);
+    };
+    const auto tokens = [&](int s, int kb) { tma_load_2d(base + s * kStage + kA, &map_x, full + 8 * s, kb * kGemmK, 0); };
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; ++i) {
             mbar_init(full + 8 * i, 1);
@@ -37,6 +50,7 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(const __grid_c
         mbar_init(done, 1);
         sts_s32(abort_flag, 0);
         fence_mbar_init();
+        for (int i = 0; i < ahead; ++i) weights(i, kb0 + i);     // before anything else of the CTA is ready
     }
     __syncwarp();
     if (warp == 1) tmem_alloc<1>(slot, kCols);
@@ -44,20 +58,8 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = (uint32_t)lds_volatile_s32(slot);
-    const int kb0 = (int)((long long)p.kblocks * rank / p.split), kb1 = (int)((long long)p.kblocks * (rank + 1) / p.split);
-    const int row0 = tile * (GATED ? 64 : 128);
-
     if (warp == 0) {
         if (lane == 0) {
-            const auto weights = [&](int s, int kb) {
-                const uint32_t sa = base + s * kStage, bar = full + 8 * s;
-                mbar_arrive_expect_tx(bar, kStage);
-                tma_load_2d(sa, &map_w0, bar, kb * kGemmK, row0);
-                if constexpr (GATED) tma_load_2d(sa + kA / 2, &map_w1, bar, kb * kGemmK, row0);
-            };
-            const auto tokens = [&](int s, int kb) { tma_load_2d(base + s * kStage + kA, &map_x, full + 8 * s, kb * kGemmK, 0); };
-            const int ahead = kb1 - kb0 < ST ? kb1 - kb0 : ST;
-            for (int i = 0; i < ahead; ++i) weights(i, kb0 + i);
             if constexpr (GATED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
             else asm volatile("griddepcontrol.wait;" ::: "memory");                                  // h is complete
             for (int i = 0; i < ahead; ++i) tokens(i, kb0 + i);
@@ -116,21 +118,25 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(const __grid_c
     else __syncthreads();
     // the ranks share the tile's tokens: a warp sums one token's row over the CTAs, in rank order
     for (int t = (int)rank + p.split * warp; t < p.n_tok; t += p.split * (kSmallThreads / 32)) {
-        float a[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int r = 0; r < p.split; ++r) {
-            const uint32_t from = base + t * 512 + (GATED ? lane * 8 : lane * 16);
+        const uint32_t from = base + t * 512 + (GATED ? lane * 8 : lane * 16);
+        float v[8][4];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {                    // every CTA's at once: one round trip instead of one per CTA
+            if (r >= p.split) break;
             const uint32_t src = p.split > 1 ? map_rank(from, r) : from;
             if constexpr (GATED) {
-                float x0, x1, x2, x3;
-                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x0), "=f"(x1) : "r"(src));
-                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x2), "=f"(x3) : "r"(src + 256));
-                a[0] += x0; a[1] += x1; a[2] += x2; a[3] += x3;
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[r][0]), "=f"(v[r][1]) : "r"(src));
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[r][2]), "=f"(v[r][3]) : "r"(src + 256));
             } else {
-                float x0, x1, x2, x3;
-                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x0), "=f"(x1), "=f"(x2), "=f"(x3) : "r"(src));
-                a[0] += x0; a[1] += x1; a[2] += x2; a[3] += x3;
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(v[r][0]), "=f"(v[r][1]), "=f"(v[r][2]), "=f"(v[r][3]) : "r"(src));
             }
         }
+        float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] += r < p.split ? v[r][i] : 0.f;
         __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out) + (long long)t * p.n;
         using B = Store<__nv_bfloat16>;
         if constexpr (GATED) {
@@ -171,15 +177,13 @@ static cudaError_t launch_small_t(const CUtensorMap &w0, const CUtensorMap &w1, 
     if (split < 1) split = 1;
     p.split = split;
     const int per = (p.kblocks + split - 1) / split;
-    // half an SM's shared memory even where there are fewer CTAs than SMs: clusters of CTAs that each want a whole SM do not
-    // all find room in the GPCs at once (2048 x 5632: 16 clusters of 8 took two rounds, 15 us instead of 7)
-    const int budget = 113 * 1024 - 1024 - 256;
-    p.stages = budget / kStage < per ? budget / kStage : per;
-    size_t ring = (size_t)p.stages * kStage;
-    if (ring < (size_t)N * 512) ring = (size_t)N * 512;  // the partial sums lie over the ring
-    // (at N <= 128 one stage holds N * 128 + 16384 bytes; the barriers lie behind the ring proper, so keep it whole stages)
-    while ((size_t)p.stages * kStage < ring) ++p.stages;
-    const size_t smem = 1024 + (size_t)p.stages * kStage + 256;
+    // Half an SM's shared memory, also where there are fewer CTAs than SMs: clusters of CTAs that each want a whole SM do not
+    // all find room in the GPCs at once (2048 x 5632: 16 clusters of 8 took two rounds, 15 us instead of 7).
+    constexpr int kExtra = 1024 + 256, kRing = (113 * 1024 - kExtra) / kStage * kStage;
+    static_assert(kRing >= N * 512 && kRing >= 2 * kStage, "the partial sums lie over the ring");
+    p.stages = kRing / kStage < per ? kRing / kStage : per;
+    while (p.stages * kStage < N * 512) ++p.stages;
+    const size_t smem = kExtra + (size_t)p.stages * kStage;
     auto kernel = ffn_small_kernel<N, GATED>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmMaxSmem);
     if (e != cudaSuccess) return e;
