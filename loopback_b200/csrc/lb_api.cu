@@ -900,28 +900,33 @@ static int make_map_part(CUtensorMap *m, void *base, long long rows, long long c
 
 struct GemmPlan {
     int tile = 0, splits = 1;
-    int m_tiles = 0, n_tiles = 0;
+    int m_tiles = 0, n_tiles = 0, m_tiles2 = 0, n_tiles2 = 0;
+    double us = 1e30;                  // estimated
 };
 
-// Tile shape and split along k of an m x n product over `blocks` blocks of 64: the least estimated time.
-static GemmPlan plan_gemm(long long m, long long n, long long blocks, bool gate, bool may_split, int sms) {
+// Tile shape and split along k of an m x n product over `blocks` blocks of 64 (and an m2 x n2 one beside it): the least
+// estimated time.
+static GemmPlan plan_gemm(long long m, long long n, long long blocks, bool gate, bool may_split, int sms, long long m2 = 0,
+                          long long n2 = 0) {
     GemmPlan best;
-    double best_us = 1e30;
     for (int i = 0; i < lb::kGemmTileCount; ++i) {
         if (g_opt.ffn_tile > 0 && g_opt.ffn_tile <= lb::kGemmTileCount && g_opt.ffn_tile - 1 != i) continue;
         const int cg = lb::kGemmTiles[i].cg, bn = lb::kGemmTiles[i].bn;
         const long long tm = 128LL * cg, tn = gate ? bn / 2 : bn, groups = sms / cg;
-        const long long mt = (m + tm - 1) / tm, nt = (n + tn - 1) / tn;
+        const long long mt = (m + tm - 1) / tm, nt = (n + tn - 1) / tn, mt2 = (m2 + tm - 1) / tm, nt2 = (n2 + tn - 1) / tn;
         const int most = !may_split || blocks < 8 ? 1 : blocks / 4 < 16 ? (int)(blocks / 4) : 16;
         const int forced = g_opt.ffn_splits <= 0 || !may_split ? 0 : g_opt.ffn_splits < most ? g_opt.ffn_splits : most;
         for (int s = forced ? forced : 1; s <= (forced ? forced : most); ++s) {
-            const double waves = (double)((mt * nt * s + groups - 1) / groups);
+            const double waves = (double)((mt * nt * s + mt2 * nt2 + groups - 1) / groups);
             // us per block of 64 of a tile, as measured with the SMs busy (a 128 x 128 tile is bound by what L2 delivers, the
             // 256-row one by the tensor cores), a launch's fixed part, and the slices' way out and in
             const double rate = cg == 2 ? 0.345 : bn == 256 ? 0.39 : 0.30;
             double us = waves * (double)((blocks + s - 1) / s) * rate + 4.5 + bn / 128. + (cg == 2 ? 1.0 : 0.0);
             if (s > 1) us += 2.0 + (double)s * m * n * 8. / 5.0e6;
-            if (us < best_us) { best_us = us; best.tile = i; best.splits = s; best.m_tiles = (int)mt; best.n_tiles = (int)nt; }
+            if (us < best.us) {
+                best.us = us; best.tile = i; best.splits = s;
+                best.m_tiles = (int)mt; best.n_tiles = (int)nt; best.m_tiles2 = (int)mt2; best.n_tiles2 = (int)nt2;
+            }
         }
     }
     return best;
@@ -932,7 +937,8 @@ struct Operand {
     long long rows, cols, ld;         // as it lies in memory
 };
 
-// One product m x n over `segs` segments of k columns each. C: `out` [m][n] (ld n), through `part` where k is split.
+// One product m x n over `segs` segments of k columns each, c[0] (through `part` where k is split); or, where the plan says so,
+// two products over the same k: a[0] b[0] -> c[0] and a[1] b[1] -> c[1].
 static int run_gemm(const char *who, int epi, int form, const GemmPlan &pl, const Operand *a, const Operand *b, const Operand *c,
                     void *kept, void *part, long long m, long long n, long long k, int segs, int act, const DeviceInfo &di,
                     cudaStream_t st) {
@@ -941,20 +947,22 @@ static int run_gemm(const char *who, int epi, int form, const GemmPlan &pl, cons
     lb::GemmParams p;
     const int cg = lb::kGemmTiles[pl.tile].cg, bn = lb::kGemmTiles[pl.tile].bn;
     int rc;
-    const bool split = pl.splits > 1;
-    for (int s = 0; s < segs; ++s)
+    const bool split = pl.splits > 1, two = pl.m_tiles2 > 0;
+    const int pairs = two ? 2 : segs;
+    for (int s = 0; s < pairs; ++s)
         if ((rc = make_map_tile(&maps.a[s], a[s].base, a[s].rows, a[s].cols, a[s].ld, form == lb::kFormMN ? 64 : 128))) return rc;
-    for (int s = 0; s < (epi == lb::kEpiGate ? 2 : segs); ++s)
+    for (int s = 0; s < (epi == lb::kEpiGate ? 2 : pairs); ++s)
         if ((rc = make_map_tile(&maps.b[s], b[s].base, b[s].rows, b[s].cols, b[s].ld,
                                 form != lb::kFormKK ? 64 : epi == lb::kEpiGate ? bn / 2 : bn / cg))) return rc;
     if (split) {
         if ((rc = make_map_part(&maps.c[0], part, m, n, pl.splits))) return rc;
     } else {
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < (epi == lb::kEpiStore && !two ? 1 : 2); ++i)
             if (c[i].base && (rc = make_map_tile(&maps.c[i], c[i].base, c[i].rows, c[i].cols, c[i].ld, 32))) return rc;
     }
     p.m = (int)m; p.n = (int)n; p.kblocks = (int)((k + 63) / 64); p.segs = segs;
-    p.m_tiles = pl.m_tiles; p.n_tiles = pl.n_tiles; p.splits = pl.splits; p.act = act; p.kept = static_cast<uint8_t *>(kept);
+    p.m_tiles = pl.m_tiles; p.n_tiles = pl.n_tiles; p.splits = pl.splits; p.m_tiles2 = pl.m_tiles2; p.n_tiles2 = pl.n_tiles2;
+    p.m2 = two ? (int)c[1].rows : 0; p.n2 = two ? (int)c[1].cols : 0; p.act = act; p.kept = static_cast<uint8_t *>(kept);
     p.err_word = di.err_word; p.wait_cycles = wait_limit();
     cudaError_t err = lb::launch_gemm(pl.tile, split ? (int)lb::kEpiPartial : epi, form, maps, p, di.sms, st);
     if (err == cudaSuccess && split)
@@ -963,7 +971,8 @@ static int run_gemm(const char *who, int epi, int form, const GemmPlan &pl, cons
 }
 
 struct FfnPlan {
-    GemmPlan up, down, dh, dx, dw_gu, dw_down;
+    GemmPlan up, down, dh, dx, dw_gu, dw_down, dw_both;
+    bool together = false;                              // both weight gradients in one launch
     size_t part = 0, bytes = 0;                         // offset of the slices in the workspace (dg | du, or h, lie before them), its size
 };
 
@@ -995,6 +1004,10 @@ static FfnPlan plan_ffn(long long t, long long d, long long f, int kind, int sms
         q.dx = plan_gemm(t, d, 2 * blocks(f), false, true, sms);
         q.dw_gu = plan_gemm(2 * f, d, blocks(t), false, true, sms);
         q.dw_down = plan_gemm(d, f, blocks(t), false, true, sms);
+        // the two weight gradients are sums over the same rows: in one launch their tiles fill the last round together
+        // (8192 x 1024 x 2816: 134 us apart)
+        q.dw_both = plan_gemm(2 * f, d, blocks(t), false, false, sms, d, f);
+        q.together = q.dw_both.us < q.dw_gu.us + q.dw_down.us;
         need(q.dx, t, d);
         need(q.dw_gu, 2 * f, d);
         need(q.dw_down, d, f);
@@ -1106,14 +1119,14 @@ int lb_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *
         const Operand cs[2] = {{dx, t, d, d}, {}};
         if ((rc = run_gemm(who, lb::kEpiStore, lb::kFormKN, q.dx, as, bs, cs, nullptr, part, t, d, f, 2, 0, di, st))) return rc;
     }
-    if (dw_gate_up) {
-        const Operand as[1] = {{dg, t, f2, f2}}, bs[1] = {{x, t, d, d}}, cs[2] = {{dw_gate_up, f2, d, d}, {}};
-        if ((rc = run_gemm(who, lb::kEpiStore, lb::kFormMN, q.dw_gu, as, bs, cs, nullptr, part, f2, d, t, 1, 0, di, st))) return rc;
-    }
-    if (dw_down) {
-        const Operand cs[2] = {{dw_down, d, f, f}, {}};
-        if ((rc = run_gemm(who, lb::kEpiStore, lb::kFormMN, q.dw_down, dys, hs, cs, nullptr, part, d, f, t, 1, 0, di, st))) return rc;
-    }
+    const Operand as[2] = {{dg, t, f2, f2}, dys[0]}, bs[2] = {{x, t, d, d}, hs[0]};
+    const Operand cs[2] = {{dw_gate_up, f2, d, d}, {dw_down, d, f, f}}, none[2] = {cs[1], {}};
+    if (dw_gate_up && dw_down && q.together)
+        return run_gemm(who, lb::kEpiStore, lb::kFormMN, q.dw_both, as, bs, cs, nullptr, part, f2, d, t, 1, 0, di, st);
+    if (dw_gate_up && (rc = run_gemm(who, lb::kEpiStore, lb::kFormMN, q.dw_gu, as, bs, cs, nullptr, part, f2, d, t, 1, 0, di, st)))
+        return rc;
+    if (dw_down && (rc = run_gemm(who, lb::kEpiStore, lb::kFormMN, q.dw_down, as + 1, bs + 1, none, nullptr, part, d, f, t, 1, 0, di, st)))
+        return rc;
     return LB_OK;
 }
 

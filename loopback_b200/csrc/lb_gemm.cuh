@@ -209,16 +209,18 @@ __device__ __forceinline__ void kept_values(const uint4 (&q)[12], int hi, int lo
 // Tiles in groups of 8 row tiles, rows fastest: the tiles in flight share both operands through L2. Splits are outermost, so
 // that they also share their range of k.
 struct TileAt {
-    int split, m, n;
+    int split, m, n, product;
 };
-__device__ __forceinline__ TileAt tile_at(long long t, const GemmParams &p) {
+__device__ __forceinline__ TileAt tile_at(int t, const GemmParams &p) {
     const int per = p.m_tiles * p.n_tiles;
     TileAt a;
-    a.split = (int)(t / per);
-    const int r = (int)(t - (long long)a.split * per), group = 8 * p.n_tiles;
-    const int g = r / group, left = p.m_tiles - 8 * g, rows = left < 8 ? left : 8, i = r - g * group;
-    a.m = 8 * g + i % rows;
+    a.product = t >= per * p.splits;
+    a.split = a.product ? 0 : t / per;
+    const int mt = a.product ? p.m_tiles2 : p.m_tiles, nt = a.product ? p.n_tiles2 : p.n_tiles;
+    const int r = a.product ? t - per * p.splits : t - a.split * per, group = 8 * nt;
+    const int g = r / group, left = mt - 8 * g, rows = left < 8 ? left : 8, i = r - g * group;
     a.n = i / rows;
+    a.m = 8 * g + i - a.n * rows;
     return a;
 }
 
@@ -257,8 +259,8 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
     tc_fence_after();
     const uint32_t tmem = (uint32_t)lds_volatile_s32(slot);
 
-    const long long tiles = (long long)p.m_tiles * p.n_tiles * p.splits;
-    const long long first = blockIdx.x / CG, step = gridDim.x / CG;
+    const int tiles = p.m_tiles * p.n_tiles * p.splits + p.m_tiles2 * p.n_tiles2;
+    const int first = blockIdx.x / CG, step = gridDim.x / CG;
     const int blocks = p.kblocks * p.segs;
 
     if (warp == 0) {
@@ -268,14 +270,15 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
             uint32_t ph = 0;
             long long issued = 0;
             bool ok = true;
-            for (long long t = first; ok && t < tiles; t += step) {
+            for (int t = first; ok && t < tiles; t += step) {
                 const TileAt at = tile_at(t, p);
                 const int kb0 = (int)((long long)blocks * at.split / p.splits), kb1 = (int)((long long)blocks * (at.split + 1) / p.splits);
                 const int m0 = (at.m * CG + (int)rank) * kGemmM;
                 const int n0 = EPI == kEpiGate ? at.n * (BN / 2) : at.n * BN + (int)rank * Sh::kBRows;
                 for (int kb = kb0; kb < kb1; ++kb) {
                     if (!(ok = mbar_wait(empty + 8 * s, ph ^ 1, wc, kDevWaitEmpty))) break;
-                    const int seg = kb >= p.kblocks, k0 = (kb - seg * p.kblocks) * kGemmK;
+                    const int half = kb >= p.kblocks, k0 = (kb - half * p.kblocks) * kGemmK;
+                    const int seg = A_MN ? at.product : half;
                     const uint32_t sa = base + s * Sh::kStageBytes, sb = sa + Sh::kABytes, bar = lead_full + 8 * s;
                     if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, CG * Sh::kStageBytes);
                     if constexpr (!A_MN) {
@@ -323,7 +326,7 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
             int s = 0, acc = 0;
             uint32_t ph = 0, aph = 0;
             bool ok = true;
-            for (long long t = first; ok && t < tiles; t += step) {
+            for (int t = first; ok && t < tiles; t += step) {
                 const TileAt at = tile_at(t, p);
                 const int kb0 = (int)((long long)blocks * at.split / p.splits), kb1 = (int)((long long)blocks * (at.split + 1) / p.splits);
                 if (!(ok = mbar_wait(tempty + 8 * acc, aph ^ 1, wc, kDevWaitTmem))) break;
@@ -371,11 +374,12 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
         if constexpr (EPI == kEpiGateBwd) {
             if (first < tiles) fetch(kept[0], tile_at(first, p), 0);
         }
-        for (long long t = first; t < tiles; t += step) {
+        for (int t = first; t < tiles; t += step) {
             const TileAt at = tile_at(t, p);
             const int row0 = (at.m * CG + (int)rank) * kGemmM + quad * 32;
             const int n0 = at.n * (EPI == kEpiGate ? BN / 2 : BN);
-            const bool rows = row0 < p.m;
+            const int limit_n = A_MN && at.product ? p.n2 : p.n;
+            const bool rows = row0 < (A_MN && at.product ? p.m2 : p.m);
             const uint32_t ta = tmem + ((uint32_t)(quad * 32) << 16) + acc * BN;
             if (!warp_wait(tfull + 8 * acc, aph, wc, kDevWaitTmem)) break;
             tc_fence_after();
@@ -383,7 +387,7 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
 #pragma unroll 1
                 for (int c = half; c < CHUNKS; c += HALVES) {
                     const int col = n0 + c * CW;
-                    const bool live = rows && col < p.n;
+                    const bool live = rows && col < limit_n;
                     const uint32_t dst = buf + turn * 4096 + mine;
                     turn ^= 1;
                     float v[CW];
@@ -409,7 +413,7 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
                     __syncwarp();
                     if (lane == 0) {
                         if (live) {
-                            if constexpr (EPI == kEpiStore) tma_store_2d(&maps.c[0], dst - mine, col, row0);
+                            if constexpr (EPI == kEpiStore) tma_store_2d(&maps.c[A_MN ? at.product : 0], dst - mine, col, row0);
                             else tma_store_3d(&maps.c[0], dst - mine, col, row0, at.split);
                         }
                         bulk_commit();
@@ -524,8 +528,9 @@ cudaError_t launch_gemm_t(const GemmMaps &maps, const GemmParams &p, int sms, cu
     auto kernel = gemm_kernel<CG, BN, EPI, A_MN, B_MN, ACT>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
     if (e != cudaSuccess) return e;
-    const long long tiles = (long long)p.m_tiles * p.n_tiles * p.splits;
+    const long long tiles = (long long)p.m_tiles * p.n_tiles * p.splits + (long long)p.m_tiles2 * p.n_tiles2;
     const long long groups = sms / CG;
+    if (tiles < 1 || tiles + groups > 0x7fffffffLL) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(CG * (tiles < groups ? tiles : groups)));
     cfg.blockDim = dim3(Sh::kThreads);

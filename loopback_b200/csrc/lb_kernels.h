@@ -229,7 +229,7 @@ enum GemmEpilogue : int {
 };
 
 struct GemmMaps {
-    CUtensorMap a[2], b[2];   // operands, one pair per segment of k (kEpiGate: b[0], b[1] are the two projections)
+    CUtensorMap a[2], b[2];   // operands, one pair per segment of k or per product (kEpiGate: b[0], b[1] are the projections)
     CUtensorMap c[2];         // results: boxes of 64 bf16 (32 fp32) columns x 32 rows
 };
 
@@ -238,6 +238,7 @@ struct GemmParams {
     int kblocks;              // blocks of 64 along k in one segment
     int segs;                 // segments of k, each with operands of its own (1 or 2)
     int m_tiles, n_tiles, splits;
+    int m2, n2, m_tiles2, n_tiles2;   // kFormMN: a second product over the same k in the same launch (m_tiles2 = 0: none)
     int act;                  // LB_ACT_*
     uint8_t *kept;            // act'(g) u and act(g) in blocks of 32 x 32 (kEpiGate: null = not kept)
     int *err_word;

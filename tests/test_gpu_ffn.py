@@ -65,6 +65,21 @@ def test_chosen_shapes(t, d, f, act):
     _check(t, d, f, act)
 
 
+@pytest.mark.parametrize("t,d,f", [(1300, 264, 1288), (3000, 1032, 520), (700, 1024, 2816)])
+def test_gradients_of_both_weights_and_of_one(t, d, f):
+    """Both weight gradients at once (one launch where that is faster) and each alone give the same values up to the order of
+    a sum split along the rows."""
+    from loopback_b200 import block
+    (x, wg, wu, wd), dy = _inputs(t, d, f, 11)
+    want = ref.ffn(*(v.detach().double() for v in (x, wg, wu, wd)), "silu", dy.double())
+    for need in ((1, 2, 3), (1, 2), (2,), (3,)):
+        ins = [v.detach().requires_grad_(i in need) for i, v in enumerate((x, wg, wu, wd))]
+        got = torch.autograd.grad(block.gated_ffn(*ins), [ins[i] for i in need], dy)
+        for i, g in zip(need, got):
+            name = ("dx", "dw_gate", "dw_up", "dw_down")[i]
+            ref.check_ffn(name, g, *want[name])
+
+
 def test_same_bits_every_run():
     a, b = _check(2500, 520, 1416), _check(2500, 520, 1416)
     for k in a:
