@@ -869,16 +869,18 @@ int lb_dropout(const void *x, void *out, int threshold, const int64_t *rng, int6
 // ---------------------------------------------------------------------------------------------------------
 // the gated feed-forward block
 // ---------------------------------------------------------------------------------------------------------
-// 2-D bf16 matrix [rows][cols], `ld` columns from row to row; boxes of 64 columns x box_rows rows, 128-byte swizzle
-static int make_map_tile(CUtensorMap *m, const void *base, long long rows, long long cols, long long ld, int box_rows) {
+// 2-D bf16 matrix [rows][cols], `ld` columns from row to row; boxes of 64 columns x box_rows rows, 128-byte swizzle (or 32
+// columns, 64-byte swizzle)
+static int make_map_tile(CUtensorMap *m, const void *base, long long rows, long long cols, long long ld, int box_rows,
+                         int box_cols = 64) {
     auto fn = encode_fn();
     if (!fn) return fail(LB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
     cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-    cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(LB_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
     return LB_OK;
@@ -958,7 +960,8 @@ static int run_gemm(const char *who, int epi, int form, const GemmPlan &pl, cons
         if ((rc = make_map_part(&maps.c[0], part, m, n, pl.splits))) return rc;
     } else {
         for (int i = 0; i < (epi == lb::kEpiStore && !two ? 1 : 2); ++i)
-            if (c[i].base && (rc = make_map_tile(&maps.c[i], c[i].base, c[i].rows, c[i].cols, c[i].ld, 32))) return rc;
+            if (c[i].base && (rc = make_map_tile(&maps.c[i], c[i].base, c[i].rows, c[i].cols, c[i].ld, 32,
+                                                    epi == lb::kEpiGate || epi == lb::kEpiGateBwd ? 32 : 64))) return rc;
     }
     p.m = (int)m; p.n = (int)n; p.kblocks = (int)((k + 63) / 64); p.segs = segs;
     p.m_tiles = pl.m_tiles; p.n_tiles = pl.n_tiles; p.splits = pl.splits; p.m_tiles2 = pl.m_tiles2; p.n_tiles2 = pl.n_tiles2;

@@ -24,13 +24,14 @@ constexpr int kGemmMaxSmem = 227 * 1024;
 template <int CG, int BN, int EPI>
 struct GemmShape {
     static constexpr bool kGated = EPI == kEpiGate || EPI == kEpiGateBwd;
-    static constexpr int kEpiWarps = kGated && CG == 2 ? 8 : 4;
+    // the gated epilogues do more per element than one tile's multiplies leave time for with 4 or 8 warps
+    static constexpr int kEpiWarps = kGated ? BN / 16 : 4;
     static constexpr int kThreads = 64 + 32 * kEpiWarps;
-    static constexpr int kBufs = 2;                                  // 4 KB result buffers of a warp
     static constexpr int kABytes = kGemmM * 128;
     static constexpr int kBRows = BN / CG;                           // of B's tile in this CTA
     static constexpr int kStageBytes = kABytes + kBRows * 128;
-    static constexpr int kStaging = kEpiWarps * kBufs * 4096;
+    static constexpr int kBuf = kGated ? 2048 : 4096;                // result box of a warp, two of them
+    static constexpr int kStaging = kEpiWarps * 2 * kBuf;
     static constexpr int kTail = 1024 + 512;                         // alignment, barriers
     static constexpr int kFit = (kGemmMaxSmem - kTail - kStaging) / kStageBytes;
     static constexpr int kStages = kFit < 8 ? kFit : 8;
@@ -133,6 +134,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
         : "r"(addr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
+    uint32_t *r = reinterpret_cast<uint32_t *>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void sts_v4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
@@ -176,30 +187,24 @@ __device__ __forceinline__ void act_both(float g, float &a, float &slope) {
 // mantissa and fp32's range; in bf16 these two would be the largest error of every gradient). The buffer is laid out as the
 // threads hold the values, in blocks of 32 rows x 32 columns: 12 pieces of 512 bytes, 16 per lane (= row), so both directions
 // are whole-line accesses without a detour through shared memory. Pieces 0-3 / 4-7: the upper halves of the two values,
-// 8-9 / 10-11: the third bytes.
+// 8-9 / 10-11: the third bytes. A step of 16 columns is two pieces of upper halves and one of third bytes for each value.
 constexpr int kKeptBlock = 12 * 512;
-__device__ __forceinline__ void keep_values(const float (&v)[32], uint8_t *dst, int hi, int lo) {
-    uint32_t low[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t a = __byte_perm(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), 0x0051);
-        const uint32_t b = __byte_perm(__float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]), 0x0051);
-        low[i] = __byte_perm(a, b, 0x5410);
-    }
+__device__ __forceinline__ void pack_kept(const float (&v)[16], uint4 &h0, uint4 &h1, uint4 &low) {
+    uint32_t l[4], h[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        uint32_t h[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = __byte_perm(__float_as_uint(v[8 * i + 2 * j]), __float_as_uint(v[8 * i + 2 * j + 1]), 0x7632);
-        st_global_v4(dst + (hi + i) * 512, make_uint4(h[0], h[1], h[2], h[3]));
+        const uint32_t a = __byte_perm(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), 0x0051);
+        const uint32_t b = __byte_perm(__float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]), 0x0051);
+        l[i] = __byte_perm(a, b, 0x5410);
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) st_global_v4(dst + (lo + i) * 512, make_uint4(low[4 * i], low[4 * i + 1], low[4 * i + 2], low[4 * i + 3]));
+    for (int i = 0; i < 8; ++i) h[i] = __byte_perm(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), 0x7632);
+    h0 = make_uint4(h[0], h[1], h[2], h[3]);
+    h1 = make_uint4(h[4], h[5], h[6], h[7]);
+    low = make_uint4(l[0], l[1], l[2], l[3]);
 }
-// values 8 i .. 8 i + 7 of one of the two, from its pieces; the lowest byte repeats the third (it was cut off)
-__device__ __forceinline__ void kept_values(const uint4 (&q)[12], int hi, int lo, int i, float (&v)[8]) {
-    const uint4 h = q[hi + i], l = q[lo + (i >> 1)];
-    const uint32_t l0 = i & 1 ? l.z : l.x, l1 = i & 1 ? l.w : l.y;
+// 8 values from their upper halves and third bytes; the lowest byte repeats the third (it was cut off)
+__device__ __forceinline__ void kept_values(const uint4 &h, uint32_t l0, uint32_t l1, float (&v)[8]) {
     v[0] = __uint_as_float(__byte_perm(h.x, l0, 0x1044)); v[1] = __uint_as_float(__byte_perm(h.x, l0, 0x3255));
     v[2] = __uint_as_float(__byte_perm(h.y, l0, 0x1066)); v[3] = __uint_as_float(__byte_perm(h.y, l0, 0x3277));
     v[4] = __uint_as_float(__byte_perm(h.z, l1, 0x1044)); v[5] = __uint_as_float(__byte_perm(h.z, l1, 0x3255));
@@ -228,7 +233,7 @@ template <int CG, int BN, int EPI, bool A_MN, bool B_MN, int ACT>
 __global__ void __launch_bounds__(GemmShape<CG, BN, EPI>::kThreads, 1)
 gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
     using Sh = GemmShape<CG, BN, EPI>;
-    constexpr int ST = Sh::kStages, EW = Sh::kEpiWarps, NB = Sh::kBufs;
+    constexpr int ST = Sh::kStages, EW = Sh::kEpiWarps;
     extern __shared__ uint8_t raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     const uint32_t staging = base + ST * Sh::kStageBytes;
@@ -350,30 +355,24 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
     } else {
         const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
         constexpr int HALVES = EW / 4;
-        const uint32_t buf = staging + ew * NB * 4096, mine = lane * 128;
-        const uint32_t sw = lane & 7;
+        const uint32_t buf = staging + ew * 2 * Sh::kBuf;
+        // a result box in shared memory: rows of 128 bytes (64 where gated), 16-byte units permuted as the copy expects them
+        const uint32_t mine = lane * (Sh::kGated ? 64 : 128), sw = Sh::kGated ? lane >> 1 & 3 : lane & 7;
         const uint32_t lead_tempty = CG == 2 ? map_rank(tempty, 0) : tempty;
         int acc = 0;
         uint32_t aph = 0;
         int turn = 0;
-        constexpr int CW = EPI == kEpiPartial ? 32 : 64;                           // columns of a result box
+        constexpr int CW = EPI == kEpiStore ? 64 : 32;                             // columns of a result box
         constexpr int CHUNKS = (EPI == kEpiGate ? BN / 2 : BN) / CW;
-        constexpr int MINE = CHUNKS / HALVES;                                      // chunks of this warp: half, half + HALVES, ..
         const int kept_cols = (p.n + 31) / 32;
-        // kEpiGateBwd: piece `i` (32 columns) of this warp's part of tile t, fetched one piece ahead, over tile borders too
-        uint4 kept[EPI == kEpiGateBwd ? 2 : 1][12];
-        const auto fetch = [&](uint4 (&q)[12], const TileAt &at, int i) {
-            const int row0 = (at.m * CG + (int)rank) * kGemmM + quad * 32;
-            const int col = at.n * BN + (half + (i >> 1) * HALVES) * 64 + (i & 1) * 32;
-            if (row0 < p.m && col < p.n) {
-                const uint8_t *src = p.kept + ((long long)(row0 >> 5) * kept_cols + (col >> 5)) * kKeptBlock + lane * 16;
-#pragma unroll
-                for (int j = 0; j < 12; ++j) q[j] = ld_global_stream_v4(src + j * 512);
+        const auto release = [&] {                                                 // the accumulator has been read
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 2) mbar_arrive_cluster(lead_tempty + 8 * acc);
+                else mbar_arrive(tempty + 8 * acc);
             }
         };
-        if constexpr (EPI == kEpiGateBwd) {
-            if (first < tiles) fetch(kept[0], tile_at(first, p), 0);
-        }
         for (int t = first; t < tiles; t += step) {
             const TileAt at = tile_at(t, p);
             const int row0 = (at.m * CG + (int)rank) * kGemmM + quad * 32;
@@ -381,6 +380,19 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
             const int limit_n = A_MN && at.product ? p.n2 : p.n;
             const bool rows = row0 < (A_MN && at.product ? p.m2 : p.m);
             const uint32_t ta = tmem + ((uint32_t)(quad * 32) << 16) + acc * BN;
+            uint8_t *kept = Sh::kGated && p.kept ? p.kept + (long long)(row0 >> 5) * kept_cols * kKeptBlock + lane * 16 : nullptr;
+            // kEpiGateBwd: the first 16 columns' kept values while the multiplies run
+            uint4 kq[EPI == kEpiGateBwd ? 2 : 1][6];
+            const auto fetch = [&](uint4 (&q)[6], int i) {                         // step i of this warp: 16 columns
+                const int col = n0 + (half + (i >> 1) * HALVES) * 32;
+                if (rows && col < p.n) {
+                    const uint8_t *src = kept + (long long)(col >> 5) * kKeptBlock + (i & 1) * 1024;
+                    q[0] = ld_global_stream_v4(src); q[1] = ld_global_stream_v4(src + 512);
+                    q[2] = ld_global_stream_v4(src + 2048); q[3] = ld_global_stream_v4(src + 2560);
+                    q[4] = ld_global_stream_v4(src - (i & 1) * 512 + 4096); q[5] = ld_global_stream_v4(src - (i & 1) * 512 + 5120);
+                }
+            };
+            if constexpr (EPI == kEpiGateBwd) fetch(kq[0], 0);
             if (!warp_wait(tfull + 8 * acc, aph, wc, kDevWaitTmem)) break;
             tc_fence_after();
             if constexpr (EPI == kEpiStore || EPI == kEpiPartial) {
@@ -419,96 +431,97 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
                         bulk_commit();
                     }
                 }
+                release();
             } else if constexpr (EPI == kEpiGate) {
-#pragma unroll 1
-                for (int c = half; c < CHUNKS; c += HALVES) {
-                    const int col = n0 + c * 64;
-                    const bool live = rows && col < p.n;
-                    const uint32_t dst = buf + turn * 4096 + mine;
-                    turn ^= 1;
-                    if (lane == 0) bulk_wait_read<1>();
-                    __syncwarp();
+                static_assert(CHUNKS == HALVES, "one box of 32 columns per warp");
+                const int col = n0 + half * 32;
+                const bool live = rows && col < p.n;
+                const uint32_t dst = buf + turn * Sh::kBuf + mine;
+                turn ^= 1;
+                if (lane == 0) bulk_wait_read<1>();
+                __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float g[32], u[32];
-                        tmem_ld32(ta + c * 64 + j * 32, g);
-                        tmem_ld32(ta + BN / 2 + c * 64 + j * 32, u);
-                        tmem_wait_ld();
-                        if (!live) continue;
+                for (int j = 0; j < 2; ++j) {
+                    float g[16], u[16];
+                    tmem_ld16(ta + half * 32 + j * 16, g);
+                    tmem_ld16(ta + BN / 2 + half * 32 + j * 16, u);
+                    tmem_wait_ld();
+                    if (j == 1) release();
+                    if (!live) continue;
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            float h[8];
+                    for (int q = 0; q < 2; ++q) {
+                        float h[8];
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                float a, slope;
-                                act_both<ACT>(g[8 * q + e], a, slope);
-                                h[e] = a * u[8 * q + e];
-                                g[8 * q + e] = a;
-                                u[8 * q + e] *= slope;
-                            }
-                            const uint4 hq = Store<__nv_bfloat16>::pack(h);
-                            sts_v4(dst + (((j * 4 + q) ^ sw) << 4), hq.x, hq.y, hq.z, hq.w);
+                        for (int e = 0; e < 8; ++e) {
+                            float a, slope;
+                            act_both<ACT>(g[8 * q + e], a, slope);
+                            h[e] = a * u[8 * q + e];
+                            g[8 * q + e] = a;
+                            u[8 * q + e] *= slope;
                         }
-                        if (p.kept && col + j * 32 < p.n) {
-                            uint8_t *to = p.kept + ((long long)(row0 >> 5) * kept_cols + ((col + j * 32) >> 5)) * kKeptBlock + lane * 16;
-                            keep_values(u, to, 0, 8);
-                            keep_values(g, to, 4, 10);
-                        }
+                        const uint4 hq = Store<__nv_bfloat16>::pack(h);
+                        sts_v4(dst + (((j * 2 + q) ^ sw) << 4), hq.x, hq.y, hq.z, hq.w);
                     }
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (live) tma_store_2d(&maps.c[0], dst - mine, col, row0);
-                        bulk_commit();
+                    if (p.kept) {
+                        uint8_t *to = kept + (long long)(col >> 5) * kKeptBlock;
+                        uint4 h0, h1, low;
+                        pack_kept(u, h0, h1, low);
+                        st_global_v4(to + j * 1024, h0);
+                        st_global_v4(to + j * 1024 + 512, h1);
+                        st_global_v4(to + 4096 + j * 512, low);
+                        pack_kept(g, h0, h1, low);
+                        st_global_v4(to + 2048 + j * 1024, h0);
+                        st_global_v4(to + 2048 + j * 1024 + 512, h1);
+                        st_global_v4(to + 5120 + j * 512, low);
                     }
                 }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    if (live) tma_store_2d(&maps.c[0], dst - mine, col, row0);
+                    bulk_commit();
+                }
             } else {
-                const TileAt next = tile_at(t + step < tiles ? t + step : t, p);
-                const bool more = t + step < tiles;
+                constexpr int STEPS = 2 * CHUNKS / HALVES;
 #pragma unroll
-                for (int i = 0; i < 2 * MINE; ++i) {
-                    const int c = half + (i >> 1) * HALVES, j = i & 1, col = n0 + c * 64;
+                for (int i = 0; i < STEPS; ++i) {
+                    const int c = half + (i >> 1) * HALVES, j = i & 1, col = n0 + c * 32;
                     const bool live = rows && col < p.n;
-                    if (i + 1 < 2 * MINE) fetch(kept[(i + 1) & 1], at, i + 1);
-                    else if (more) fetch(kept[0], next, 0);
-                    float v[32];
-                    tmem_ld32(ta + c * 64 + j * 32, v);
+                    float v[16];
+                    tmem_ld16(ta + c * 32 + j * 16, v);
+                    if (i + 1 < STEPS) fetch(kq[(i + 1) & 1], i + 1);
                     if (j == 0 && lane == 0) bulk_wait_read<0>();
                     tmem_wait_ld();
                     __syncwarp();
+                    if (i + 1 == STEPS) release();
                     if (live) {
+                        const uint4 (&k)[6] = kq[i & 1];
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
+                        for (int q = 0; q < 2; ++q) {
                             float a[8], b[8];
-                            kept_values(kept[i & 1], 0, 8, q, a);
-                            kept_values(kept[i & 1], 4, 10, q, b);
+                            kept_values(k[q], q ? k[4].z : k[4].x, q ? k[4].w : k[4].y, a);
+                            kept_values(k[2 + q], q ? k[5].z : k[5].x, q ? k[5].w : k[5].y, b);
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
                                 a[e] *= v[8 * q + e];
                                 b[e] *= v[8 * q + e];
                             }
-                            const uint32_t o = buf + mine + (((j * 4 + q) ^ sw) << 4);
+                            const uint32_t o = buf + mine + (((j * 2 + q) ^ sw) << 4);
                             const uint4 aq = Store<__nv_bfloat16>::pack(a), bq = Store<__nv_bfloat16>::pack(b);
                             sts_v4(o, aq.x, aq.y, aq.z, aq.w);
-                            sts_v4(o + 4096, bq.x, bq.y, bq.z, bq.w);
+                            sts_v4(o + Sh::kBuf, bq.x, bq.y, bq.z, bq.w);
                         }
-                        if (j == 1) fence_async_smem();
                     }
                     if (j == 1) {
+                        fence_async_smem();
                         __syncwarp();
                         if (lane == 0 && live) {
                             tma_store_2d(&maps.c[0], buf, col, row0);
-                            tma_store_2d(&maps.c[1], buf + 4096, col, row0);
+                            tma_store_2d(&maps.c[1], buf + Sh::kBuf, col, row0);
                             bulk_commit();
                         }
                     }
                 }
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (CG == 2) mbar_arrive_cluster(lead_tempty + 8 * acc);
-                else mbar_arrive(tempty + 8 * acc);
             }
             if (++acc == 2) { acc = 0; aph ^= 1; }
         }

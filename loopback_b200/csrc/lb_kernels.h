@@ -230,7 +230,7 @@ enum GemmEpilogue : int {
 
 struct GemmMaps {
     CUtensorMap a[2], b[2];   // operands, one pair per segment of k or per product (kEpiGate: b[0], b[1] are the projections)
-    CUtensorMap c[2];         // results: boxes of 64 bf16 (32 fp32) columns x 32 rows
+    CUtensorMap c[2];         // results: boxes of 64 bf16 columns x 32 rows; 32 where gated (64-byte swizzle) or fp32
 };
 
 struct GemmParams {
