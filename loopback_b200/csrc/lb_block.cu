@@ -114,6 +114,27 @@ __device__ __forceinline__ float row_sum(float v, int wpt, int grp, int wl, int 
     return t;
 }
 
+__device__ __forceinline__ float3 row_sums(float3 v, int wpt, int grp, int wl, int lane, float (*slots)[3][kBlkWarps], int &turn) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+        v.z += __shfl_xor_sync(0xffffffffu, v.z, o);
+    }
+    if (wpt == 1) return v;
+    float (*s)[kBlkWarps] = slots[turn];
+    turn ^= 1;
+    if (lane < 3) s[lane][grp * wpt + wl] = lane == 0 ? v.x : lane == 1 ? v.y : v.z;
+    named_bar_sync(1 + grp, wpt * 32);
+    float3 t = make_float3(0.f, 0.f, 0.f);
+    for (int i = 0; i < wpt; ++i) {
+        t.x += s[0][grp * wpt + i];
+        t.y += s[1][grp * wpt + i];
+        t.z += s[2][grp * wpt + i];
+    }
+    return t;
+}
+
 // Shared memory of both kernels: the ring [array][2 rows ahead][FR][thread] of 16 bytes, then the two channel tables; the
 // backward's column sums take the ring's place at the end.
 constexpr int kSlot = kBlkThreads * 16;
@@ -265,7 +286,7 @@ template <typename T, typename W, int FR, bool RES>
 __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && sizeof(T) == 4) ? 2 : 1) block_bwd_kernel(const BlockParams p) {
     using S = Store<T>;
     constexpr int VEC = S::kVec, P = S::kPairs;
-    __shared__ float slots[2][kBlkWarps];
+    __shared__ float slots[2][kBlkWarps], slots3[2][3][kBlkWarps];
     extern __shared__ __align__(16) uint8_t dyn[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int wpt = p.wpt, groups = kBlkWarps / wpt, grp = warp / wpt, wl = warp % wpt;
@@ -335,86 +356,94 @@ __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && si
         const float gt = RES && p.gate_kind == kGateToken ? S::load1(static_cast<const T *>(p.gate) + tok) : 1.f;
         const float2 ry2 = splat(ry), ro2 = splat(ro);
         cp_async_wait<1>();
-        float2 D[FR][P], oh[FR][P], yh[RES ? FR : 1][P];
+        float2 D[FR][P], oh[FR][P];
         uint32_t words[RES ? FR : 1][P];
-        float2 acc = splat(0.f);
-        // the gradient of o through its norm
+        // One exchange per row: with t = w' du and b = w g m yh, the sums of t oh, b (dout + r_o t) and b oh give both means,
+        // mean(t oh) and the sum of b D that the norm after the block and the token gate's gradient want
+        float2 s1 = splat(0.f), s2 = splat(0.f), s3 = splat(0.f);
 #pragma unroll
         for (int k = 0; k < FR; ++k) {
-            const int f = f0 + 32 * k;
-            const bool in = f < p.frags;
+            const bool in = f0 + 32 * k < p.frags;
 #pragma unroll
             for (int i = 0; i < P; ++i) D[k][i] = oh[k][i] = splat(0.f);
+            float2 b[P], c[P];
             if constexpr (RES) {
-                S::unpack2(in ? lds_v4(slot(stage, 2, k)) : make_uint4(0, 0, 0, 0), yh[k]);
-#pragma unroll
-                for (int i = 0; i < P; ++i) yh[k][i] = __fmul2_rn(yh[k][i], ry2);
-                if (in && p.drop.threshold) drop_words<P>(words[k], (unsigned long long)(row + k * 32 * VEC), seed, offset);
-            }
-            if (in && du) {
-                float2 c[P];
-                S::unpack2(lds_v4(slot(stage, 1, k)), oh[k]);
-                if constexpr (RES) {
-                    float2 b[P];
+                if (in) {
+                    S::unpack2(lds_v4(slot(stage, 2, k)), b);
                     channel_pairs<P>(c, tab_wg + k * 512, plane);
 #pragma unroll
-                    for (int i = 0; i < P; ++i) b[i] = __fmul2_rn(c[i], yh[k][i]);
+                    for (int i = 0; i < P; ++i) b[i] = __fmul2_rn(c[i], __fmul2_rn(b[i], ry2));
                     if (gate) {
                         S::unpack2(lds_v4(slot(stage, 4, k)), c);
 #pragma unroll
                         for (int i = 0; i < P; ++i) b[i] = __fmul2_rn(b[i], c[i]);
                     }
-                    if (p.drop.threshold) drop_pairs<P>(b, words[k], p.drop.threshold);
+                    if (p.drop.threshold) {
+                        drop_words<P>(words[k], (unsigned long long)(row + k * 32 * VEC), seed, offset);
+                        drop_pairs<P>(b, words[k], p.drop.threshold);
+                    }
+                    if (dout) {
+                        S::unpack2(lds_v4(slot(stage, 3, k)), c);
 #pragma unroll
-                    for (int i = 0; i < P; ++i) oh[k][i] = __ffma2_rn(splat(s * gt), b[i], oh[k][i]);
+                        for (int i = 0; i < P; ++i) s2 = __ffma2_rn(b[i], c[i], s2);
+                    }
                 }
+            }
+            if (in && du) {
                 float2 uu[P];
+                S::unpack2(lds_v4(slot(stage, 1, k)), oh[k]);
                 S::unpack2(lds_v4(slot(stage, 0, k)), uu);
                 channel_pairs<P>(c, tab_w2 + k * 512, plane);
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
+                    if constexpr (RES) oh[k][i] = __ffma2_rn(splat(s * gt), b[i], oh[k][i]);
                     oh[k][i] = __fmul2_rn(oh[k][i], ro2);
                     colB[k][i] = __ffma2_rn(uu[i], oh[k][i], colB[k][i]);
                     D[k][i] = __fmul2_rn(c[i], uu[i]);
-                    acc = __ffma2_rn(D[k][i], oh[k][i], acc);
+                    s1 = __ffma2_rn(D[k][i], oh[k][i], s1);
+                    if constexpr (RES) {
+                        s2 = __ffma2_rn(b[i], __fmul2_rn(ro2, D[k][i]), s2);
+                        s3 = __ffma2_rn(b[i], oh[k][i], s3);
+                    }
                 }
             }
-        }
-        if (du) {
-            const float2 c1 = splat(-row_sum(acc.x + acc.y, wpt, grp, wl, lane, slots, turn) * inv_d);
-#pragma unroll
-            for (int k = 0; k < FR; ++k)
-#pragma unroll
-                for (int i = 0; i < P; ++i) D[k][i] = __fmul2_rn(ro2, __ffma2_rn(c1, oh[k][i], D[k][i]));
         }
         if constexpr (!RES) {
             fetch(stage, tok + 2 * step);
+            const float2 c1 = splat(-row_sum(s1.x + s1.y, wpt, grp, wl, lane, slots, turn) * inv_d);
 #pragma unroll
             for (int k = 0; k < FR; ++k) {
-                const int f = f0 + 32 * k;
-                if (f < p.frags && dx) st_global_v4(dx + row + k * 32 * VEC, S::pack2v(D[k]));
+                if (f0 + 32 * k >= p.frags || !dx) continue;
+#pragma unroll
+                for (int i = 0; i < P; ++i) D[k][i] = __fmul2_rn(ro2, __ffma2_rn(c1, oh[k][i], D[k][i]));
+                st_global_v4(dx + row + k * 32 * VEC, S::pack2v(D[k]));
             }
         } else {
-            float2 sum = splat(0.f);                     // of w g (m D) yh: the token gate's gradient and the norm's mean
+            float3 sums = row_sums(make_float3(s1.x + s1.y, s2.x + s2.y, s3.x + s3.y), wpt, grp, wl, lane, slots3, turn);
+            const float mean = sums.x * inv_d, S1 = fmaf(-ro * mean, sums.z, sums.y);
+            if (p.gate_kind == kGateToken && p.dgate && wl == 0 && lane == 0) S::store1(static_cast<T *>(p.dgate) + tok, s * S1);
+            const float2 c1 = splat(-mean), k1 = splat(s * gt * ry), c2 = splat(w ? -S1 * inv_d : 0.f);
 #pragma unroll
             for (int k = 0; k < FR; ++k) {
-                const int f = f0 + 32 * k;
-                if (f >= p.frags) continue;
-                if (dout) {
-                    float2 v[P];
-                    S::unpack2(lds_v4(slot(stage, 3, k)), v);
+                if (f0 + 32 * k >= p.frags) continue;
+                float2 v[P], yh[P];
+                if (dout) S::unpack2(lds_v4(slot(stage, 3, k)), v);
 #pragma unroll
-                    for (int i = 0; i < P; ++i) D[k][i] = __fadd2_rn(D[k][i], v[i]);
+                for (int i = 0; i < P; ++i) {
+                    D[k][i] = __ffma2_rn(c1, oh[k][i], D[k][i]);
+                    D[k][i] = dout ? __ffma2_rn(ro2, D[k][i], v[i]) : __fmul2_rn(ro2, D[k][i]);
                 }
                 if (dx) st_global_v4(dx + row + k * 32 * VEC, S::pack2v(D[k]));
                 if (p.drop.threshold) drop_pairs<P>(D[k], words[k], p.drop.threshold);
-                float2 c[P];
-                channel_pairs<P>(c, tab_wg + k * 512, plane);
+                S::unpack2(lds_v4(slot(stage, 2, k)), yh);
+#pragma unroll
+                for (int i = 0; i < P; ++i) yh[i] = __fmul2_rn(yh[i], ry2);
+                channel_pairs<P>(v, tab_wg + k * 512, plane);
                 if (gate) {
                     float2 g[P];
                     if (p.dgate) {
 #pragma unroll
-                        for (int i = 0; i < P; ++i) g[i] = __fmul2_rn(splat(s), __fmul2_rn(c[i], __fmul2_rn(D[k][i], yh[k][i])));
+                        for (int i = 0; i < P; ++i) g[i] = __fmul2_rn(splat(s), __fmul2_rn(v[i], __fmul2_rn(D[k][i], yh[i])));
                         st_global_v4(static_cast<T *>(p.dgate) + row + k * 32 * VEC, S::pack2v(g));
                     }
                     S::unpack2(lds_v4(slot(stage, 4, k)), g);
@@ -424,26 +453,12 @@ __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && si
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
                     const float2 a = p.gate_kind == kGateToken ? __fmul2_rn(splat(gt), D[k][i]) : D[k][i];
-                    colA[k][i] = __ffma2_rn(a, yh[k][i], colA[k][i]);
-                    D[k][i] = __fmul2_rn(D[k][i], c[i]);
-                    sum = __ffma2_rn(D[k][i], yh[k][i], sum);
+                    colA[k][i] = __ffma2_rn(a, yh[i], colA[k][i]);
+                    D[k][i] = __fmul2_rn(k1, __ffma2_rn(c2, yh[i], __fmul2_rn(D[k][i], v[i])));
                 }
+                if (dy) st_global_v4(dy + row + k * 32 * VEC, S::pack2v(D[k]));
             }
             fetch(stage, tok + 2 * step);
-            float S1 = sum.x + sum.y;
-            if (w || p.gate_kind == kGateToken) S1 = row_sum(S1, wpt, grp, wl, lane, slots, turn);
-            if (p.gate_kind == kGateToken && p.dgate && wl == 0 && lane == 0) S::store1(static_cast<T *>(p.dgate) + tok, s * S1);
-            if (dy) {
-                const float2 k1 = splat(s * gt * ry), c2 = splat(w ? -S1 * inv_d : 0.f);
-#pragma unroll
-                for (int k = 0; k < FR; ++k) {
-                    const int f = f0 + 32 * k;
-                    if (f >= p.frags) continue;
-#pragma unroll
-                    for (int i = 0; i < P; ++i) D[k][i] = __fmul2_rn(k1, __ffma2_rn(c2, yh[k][i], D[k][i]));
-                    st_global_v4(dy + row + k * 32 * VEC, S::pack2v(D[k]));
-                }
-            }
         }
     }
     if (!p.part) return;
@@ -605,7 +620,7 @@ static int registers_of(const void *kernel) {
 }
 static int resident(int regs, size_t smem) {
     const int by_regs = 65536 / (kBlkWarps * ((regs * 32 + 255) / 256 * 256));
-    const int by_smem = (int)((size_t)(228 * 1024) / (smem + 64 + 1024));
+    const int by_smem = (int)((size_t)(228 * 1024) / (smem + 256 + 1024));
     const int n = by_regs < by_smem ? by_regs : by_smem;
     return n < 1 ? 1 : n > 8 ? 8 : n;
 }
@@ -613,8 +628,16 @@ static int resident(int regs, size_t smem) {
 template <typename T, typename W, bool RES>
 static cudaError_t launch_block_t(BlockParams p, bool bwd, int sms, cudaStream_t stream) {
     int fr;
-    const int most = p.most_frags ? p.most_frags : 4;
-    if (!block_shape(p.frags, p.n_tok, sms, most, &fr, &p.wpt)) return cudaErrorInvalidValue;
+    if (!block_shape(p.frags, p.n_tok, sms, p.most_frags ? p.most_frags : 4, &fr, &p.wpt)) return cudaErrorInvalidValue;
+    if (bwd && RES && !p.most_frags && fr > 2) {
+        // the residual's backward holds the most per fragment: two per lane let a second CTA onto the SM (32768 x 1024 bf16:
+        // 113 us instead of 120), unless that leaves many lanes idle (1536 columns: three per lane, 130 us instead of 136)
+        int fr2, wpt2;
+        if (block_shape(p.frags, p.n_tok, sms, 2, &fr2, &wpt2) && fr2 * wpt2 * 10 <= fr * p.wpt * 12) {
+            fr = fr2;
+            p.wpt = wpt2;
+        }
+    }
     const int groups = kBlkWarps / p.wpt;
     const bool full = p.gate_kind == kGateFull;
     const int arrays = bwd ? (RES ? 4 + full : 2) : (RES ? 2 + full : 1);
