@@ -15,10 +15,11 @@ separate PyTorch operations between their reads (looped_transformer.py, the bloc
 from __future__ import annotations
 
 import torch
+from torch import nn
 
 from . import _lib
 
-__all__ = ["block_norm", "block_residual", "dropout", "gated_ffn"]
+__all__ = ["block_norm", "block_residual", "dropout", "gated_ffn", "FeedForwardBlock"]
 
 _ACTS = {"silu": 0, "gelu": 1}
 
@@ -87,3 +88,45 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if act not in _ACTS:
         raise ValueError(f"loopback_b200.gated_ffn: act is one of {sorted(_ACTS)}, got {act!r}")
     return _lib.torch_ops().gated_ffn(x, w_gate, w_up, w_down, _ACTS[act])
+
+
+class FeedForwardBlock(nn.Module):
+    """A feed-forward block between two reads, on the operators above:
+
+        out = x + scale * gate * dropout(norm_after(ffn(norm(x))))
+
+    `post_norm` adds the norm after the block, `gate` a learned vector per channel (ones at first), `scale` the residual
+    scale (a number; a learned one with `learn_scale`), `p` the dropout of the branch, applied in training. Its result is
+    the proposal `cell.combine` takes and the first argument of `DattnStack.write`."""
+
+    def __init__(self, dim: int, hidden: int, act: str = "silu", *, post_norm: bool = False, gate: bool = False, scale: float = 1.0,
+                 learn_scale: bool = False, p: float = 0.0, eps: float = 1e-6, device=None, dtype=torch.bfloat16):
+        super().__init__()
+        if act not in _ACTS:
+            raise ValueError(f"loopback_b200.FeedForwardBlock: act is one of {sorted(_ACTS)}, got {act!r}")
+        if dim < 1 or hidden < 1 or dim % 8 or hidden % 8:
+            raise ValueError(f"loopback_b200.FeedForwardBlock: dim and hidden are multiples of 8, got {dim} and {hidden}")
+        _threshold("FeedForwardBlock", p)
+        make = dict(device=device, dtype=dtype)
+        self.act, self.p, self.eps = act, float(p), float(eps)
+        self.norm = nn.Parameter(torch.ones(dim, **make))
+        self.norm_after = nn.Parameter(torch.ones(dim, **make)) if post_norm else None
+        self.gate = nn.Parameter(torch.ones(dim, **make)) if gate else None
+        self.scale = nn.Parameter(torch.full((1,), float(scale), device=device)) if learn_scale else float(scale)
+        self.w_gate = nn.Parameter(torch.empty(hidden, dim, **make))
+        self.w_up = nn.Parameter(torch.empty(hidden, dim, **make))
+        self.w_down = nn.Parameter(torch.empty(dim, hidden, **make))
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        with torch.no_grad():
+            for w in (self.w_gate, self.w_up, self.w_down):
+                w.normal_(0.0, w.shape[1] ** -0.5)
+
+    def forward(self, x: torch.Tensor, normed=None, next_weight=None, rng=None):
+        """out, or (out, norm of out by `next_weight`). `normed`: norm(x), where the previous block already formed it (its
+        `next_weight` was this block's `norm`). `rng`: see `dropout`; needed in training with p > 0."""
+        u = block_norm(x, self.norm, self.eps) if normed is None else normed
+        y = gated_ffn(u, self.w_gate, self.w_up, self.w_down, self.act)
+        return block_residual(x, y, self.norm_after, gate=self.gate, scale=self.scale, next_weight=next_weight, eps=self.eps,
+                              p=self.p if self.training else 0.0, rng=rng)

@@ -9,9 +9,18 @@ import block_reference as ref
 def test_no_cpu_path():
     from loopback_b200 import block
     x, w = torch.zeros(2, 64), torch.ones(64)
-    for call in (lambda: block.block_norm(x, w), lambda: block.block_residual(x, x, w), lambda: block.dropout(x, 0.5, (1, 2))):
+    b = torch.zeros(64, 64, dtype=torch.bfloat16)
+    for call in (lambda: block.block_norm(x, w), lambda: block.block_residual(x, x, w), lambda: block.dropout(x, 0.5, (1, 2)),
+                 lambda: block.gated_ffn(b, b, b, b), lambda: block.FeedForwardBlock(64, 128)(b)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+    for bad in (lambda: block.FeedForwardBlock(60, 128), lambda: block.FeedForwardBlock(64, 0), lambda: block.FeedForwardBlock(64, 64, "relu"),
+                lambda: block.FeedForwardBlock(64, 64, p=1.0), lambda: block.gated_ffn(b, b, b, b, act="tanh")):
+        with pytest.raises(ValueError):
+            bad()
+    m = block.FeedForwardBlock(64, 128, post_norm=True, gate=True, learn_scale=True)
+    assert {n: tuple(v.shape) for n, v in m.named_parameters()} == {
+        "norm": (64,), "norm_after": (64,), "gate": (64,), "scale": (1,), "w_gate": (128, 64), "w_up": (128, 64), "w_down": (64, 128)}
 
 
 def test_argument_validation_needs_no_gpu():
@@ -37,6 +46,14 @@ def test_argument_validation_needs_no_gpu():
                                    None, 4, 64, bf, bf, None)
     assert resb(dout=None) == -1 and resb(du=a) == -1 and resb(w=a) == -1 and resb(dw=a) == -1 and resb(dscale=a) == -1
     assert resb(dgate=a) == -1
+    ffn = lambda x=a, h=None, kept=None, ws=a, t=4, d=64, f=64, act=0, dt=bf: lib.lb_ffn_fwd(  # noqa: E731
+        x, a, a, a, a, h, kept, ws, 1 << 30, t, d, f, act, dt, None)
+    assert ffn(x=None) == -1 and ffn(ws=None) == -1 and ffn(kept=a) == -1 and ffn(act=2) == -1 and ffn(t=-1) == -1 and ffn(f=0) == -1
+    assert ffn(d=60) == -2 and ffn(f=12) == -2 and ffn(x=odd) == -2 and ffn(dt=f32) == -3 and ffn(f=(1 << 20) + 8) == -3
+    assert ffn(t=(1 << 31) - 8) == -3
+    ffnb = lambda dy=a, h=a, kept=a, d=64, dt=bf: lib.lb_ffn_bwd(a, a, a, a, h, kept, dy, a, a, a, a, 1 << 30, 4, d, 64, dt, None)  # noqa: E731
+    assert ffnb(dy=None) == -1 and ffnb(h=None) == -1 and ffnb(kept=None) == -1 and ffnb(dy=odd) == -2 and ffnb(d=4) == -2 and ffnb(dt=f32) == -3
+    assert lib.lb_ffn_kept_bytes(33, 40) >= 2 * 2 * 6144 and lib.lb_ffn_kept_bytes(3, 4) == 0 and lib.lb_ffn_workspace_bytes(4, 64, 64, 7) == 0
     drop = lambda x, o, n=8, thr=1, dt=bf: lib.lb_dropout(x, o, thr, None, 0, 0, None, n, dt, None)  # noqa: E731
     assert drop(None, a) == -1 and drop(a, a) == -1 and drop(odd, a) == -2 and drop(a, a + 16, n=-1) == -1
     assert drop(a, a + 16, thr=70000) == -1 and drop(a, a + 16, dt=3) == -1
