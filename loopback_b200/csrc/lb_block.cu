@@ -18,6 +18,7 @@
 // there as fp32. All arithmetic is fp32, in pairs (fma.rn.f32x2), with one rounding at each store.
 #include "lb_common.cuh"
 #include "lb_kernels.h"
+#include "lb_launch.cuh"
 
 namespace lb {
 
@@ -29,26 +30,43 @@ constexpr int kBlkWarps = kBlkThreads / 32;
 // counter (group, offset) and key seed. A group is 8 consecutive elements; element j of it takes half j (low half first) of
 // the four words, 16 bits: one call serves a 16-byte fragment of bf16, at half the integer work of a word per element.
 // ---------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint4 philox4x32_10(unsigned long long group, unsigned long long offset, unsigned long long seed) {
+// The ten rounds' keys (seed + r times the two constants) come from where the kernel has room: added up as they are needed
+// (integer pipe), kept in registers, or from shared memory (k0, k1 of round 0, 1, ..: 20 words, broadcast loads).
+struct KeysAdded {
+    uint32_t k0, k1;
+    __device__ __forceinline__ uint2 at(int r) const { return make_uint2(k0 + r * 0x9E3779B9u, k1 + r * 0xBB67AE85u); }
+};
+struct KeysHeld {
+    uint32_t k0[10], k1[10];
+    __device__ __forceinline__ uint2 at(int r) const { return make_uint2(k0[r], k1[r]); }
+};
+struct KeysShared {
+    uint32_t base;
+    __device__ __forceinline__ uint2 at(int r) const {
+        uint2 k;
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(k.x), "=r"(k.y) : "r"(base + r * 8));
+        return k;
+    }
+};
+template <typename Keys>
+__device__ __forceinline__ uint4 philox4x32_10(unsigned long long group, unsigned long long offset, const Keys &keys) {
     uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32), c2 = (uint32_t)offset, c3 = (uint32_t)(offset >> 32);
-    uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
+        const uint2 k = keys.at(r);
         const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;
-        c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+        c0 = (uint32_t)(b >> 32) ^ c1 ^ k.x;
         c1 = (uint32_t)b;
-        c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        c2 = (uint32_t)(a >> 32) ^ c3 ^ k.y;
         c3 = (uint32_t)a;
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
     }
     return make_uint4(c0, c1, c2, c3);
 }
 
 // The words that decide over the fragment at linear index `e` (a multiple of 2 P), one per pair of elements
-template <int P>
-__device__ __forceinline__ void drop_words(uint32_t (&w)[P], unsigned long long e, unsigned long long seed, unsigned long long offset) {
-    const uint4 q = philox4x32_10(e >> 3, offset, seed);
+template <int P, typename Keys>
+__device__ __forceinline__ void drop_words(uint32_t (&w)[P], unsigned long long e, const Keys &keys, unsigned long long offset) {
+    const uint4 q = philox4x32_10(e >> 3, offset, keys);
     if constexpr (P == 4) {
         w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
     } else {
@@ -68,9 +86,14 @@ __device__ __forceinline__ void drop_pairs(float2 (&v)[P], const uint32_t (&w)[P
     }
 }
 
+// the pair in use, which also goes to rng_used
 __device__ __forceinline__ void drop_state(const DropParams &dp, unsigned long long &seed, unsigned long long &offset) {
     seed = dp.rng ? (unsigned long long)dp.rng[0] : (unsigned long long)dp.seed;
     offset = dp.rng ? (unsigned long long)dp.rng[1] : (unsigned long long)dp.offset;
+    if (dp.rng_used && blockIdx.x == 0 && threadIdx.x == 0) {
+        dp.rng_used[0] = (long long)seed;
+        dp.rng_used[1] = (long long)offset;
+    }
 }
 
 __device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
@@ -140,7 +163,8 @@ __device__ __forceinline__ float3 row_sums(float3 v, int wpt, int grp, int wl, i
 constexpr int kSlot = kBlkThreads * 16;
 __host__ __device__ constexpr int ring_bytes(int arrays, int fr) { return 2 * arrays * fr * kSlot; }
 
-template <typename T, typename W, int FR, bool RES>
+// FORM 1: neither dropout nor a gate per element, known when compiled; 0: whatever the parameters say.
+template <typename T, typename W, int FR, bool RES, int FORM>
 __global__ void __launch_bounds__(kBlkThreads) block_fwd_kernel(const BlockParams p) {
     using S = Store<T>;
     constexpr int VEC = S::kVec, P = S::kPairs;
@@ -149,7 +173,7 @@ __global__ void __launch_bounds__(kBlkThreads) block_fwd_kernel(const BlockParam
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int wpt = p.wpt, groups = kBlkWarps / wpt, grp = warp / wpt, wl = warp % wpt;
     const T *x = static_cast<const T *>(p.x), *y = static_cast<const T *>(p.y);
-    const T *gate = p.gate_kind == kGateFull ? static_cast<const T *>(p.gate) : nullptr;
+    const T *gate = FORM == 0 && p.gate_kind == kGateFull ? static_cast<const T *>(p.gate) : nullptr;
     const W *w = static_cast<const W *>(p.w), *w2 = static_cast<const W *>(p.w_next);
     T *out = static_cast<T *>(p.out), *u = static_cast<T *>(p.u);
     const int arrays = RES ? (gate ? 3 : 2) : 1;
@@ -188,14 +212,10 @@ __global__ void __launch_bounds__(kBlkThreads) block_fwd_kernel(const BlockParam
     }
     const float s = RES ? (p.scale_dev ? *p.scale_dev : p.scale) * p.drop.keep_scale : 0.f;
     const float inv_d = 1.f / (float)p.d;
+    const bool drop = RES && FORM == 0 && p.drop.threshold != 0;
     unsigned long long seed = 0, offset = 0;
-    if (RES && p.drop.threshold) {
-        drop_state(p.drop, seed, offset);
-        if (p.drop.rng_used && blockIdx.x == 0 && threadIdx.x == 0) {
-            p.drop.rng_used[0] = (long long)seed;
-            p.drop.rng_used[1] = (long long)offset;
-        }
-    }
+    if (drop) drop_state(p.drop, seed, offset);
+    const KeysAdded keys{(uint32_t)seed, (uint32_t)(seed >> 32)};
     __syncthreads();
     int turn = 0, stage = 0;
     for (; tok < p.n_tok; tok += step, stage ^= 1) {
@@ -240,9 +260,9 @@ __global__ void __launch_bounds__(kBlkThreads) block_fwd_kernel(const BlockParam
 #pragma unroll
                         for (int i = 0; i < P; ++i) b[i] = __fmul2_rn(b[i], c[i]);
                     }
-                    if (p.drop.threshold) {
+                    if (drop) {
                         uint32_t words[P];
-                        drop_words<P>(words, (unsigned long long)(row + k * 32 * VEC), seed, offset);
+                        drop_words<P>(words, (unsigned long long)(row + k * 32 * VEC), keys, offset);
                         drop_pairs<P>(b, words, p.drop.threshold);
                     }
                     S::unpack2(lds_v4(slot(stage, 0, k)), o[k]);
@@ -282,19 +302,23 @@ __global__ void __launch_bounds__(kBlkThreads) block_fwd_kernel(const BlockParam
 }
 
 // Per-CTA column sums leave through p.part[CTA][2][d] (A, then B); block_param_kernel adds the CTAs' rows in a fixed order.
-template <typename T, typename W, int FR, bool RES>
+// FORM 1 / 2: both upstream gradients, no gate per element, without / with dropout, known when compiled; 0: whatever the
+// parameters say.
+template <typename T, typename W, int FR, bool RES, int FORM>
 __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && sizeof(T) == 4) ? 2 : 1) block_bwd_kernel(const BlockParams p) {
     using S = Store<T>;
     constexpr int VEC = S::kVec, P = S::kPairs;
     __shared__ float slots[2][kBlkWarps], slots3[2][3][kBlkWarps];
+    __shared__ __align__(16) uint32_t keys_[20];
     extern __shared__ __align__(16) uint8_t dyn[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int wpt = p.wpt, groups = kBlkWarps / wpt, grp = warp / wpt, wl = warp % wpt;
     const T *x = static_cast<const T *>(p.x), *y = static_cast<const T *>(p.y);
     const T *dout = static_cast<const T *>(p.d_out), *du = static_cast<const T *>(p.d_u);
-    const T *gate = p.gate_kind == kGateFull ? static_cast<const T *>(p.gate) : nullptr;
+    const T *gate = FORM == 0 && p.gate_kind == kGateFull ? static_cast<const T *>(p.gate) : nullptr;
     const W *w = static_cast<const W *>(p.w), *w2 = static_cast<const W *>(p.w_next);
     T *dx = static_cast<T *>(p.dx), *dy = static_cast<T *>(p.dy);
+    const bool has_u = FORM != 0 || du != nullptr, has_out = FORM != 0 || dout != nullptr;
     // arrays of the ring: du, x, then y, dout, gate
     const int arrays = RES ? (gate ? 5 : 4) : 2;
     const int f0 = wl * FR * 32 + lane;                  // this lane's fragments: f0, f0 + 32, ..
@@ -310,13 +334,13 @@ __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && si
             for (int k = 0; k < FR; ++k) {
                 const int f = f0 + 32 * k;
                 if (f < p.frags) {
-                    if (du) {
+                    if (has_u) {
                         cp_async16(slot(stage, 0, k), du + row + k * 32 * VEC);
                         cp_async16(slot(stage, 1, k), x + row + k * 32 * VEC);
                     }
                     if constexpr (RES) {
                         cp_async16(slot(stage, 2, k), y + row + k * 32 * VEC);
-                        if (dout) cp_async16(slot(stage, 3, k), dout + row + k * 32 * VEC);
+                        if (has_out) cp_async16(slot(stage, 3, k), dout + row + k * 32 * VEC);
                         if (gate) cp_async16(slot(stage, 4, k), gate + row + k * 32 * VEC);
                     }
                 }
@@ -330,14 +354,21 @@ __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && si
     fetch(1, tok + step);
     if constexpr (RES) {
         stage_channels<W, VEC>(tab, w, p.gate_kind == kGateChannel ? static_cast<const W *>(p.gate) : nullptr, p.d, p.frags);
-        if (du) stage_channels<W, VEC>(tab + p.frags * VEC, w2, nullptr, p.d, p.frags);
+        if (has_u) stage_channels<W, VEC>(tab + p.frags * VEC, w2, nullptr, p.d, p.frags);
     } else {
         stage_channels<W, VEC>(tab, w2, nullptr, p.d, p.frags);
     }
     const float s = RES ? (p.scale_dev ? *p.scale_dev : p.scale) * p.drop.keep_scale : 0.f;
     const float inv_d = 1.f / (float)p.d;
+    const bool drop = RES && (FORM == 0 ? p.drop.threshold != 0 : FORM == 2);
     unsigned long long seed = 0, offset = 0;
-    if (RES && p.drop.threshold) drop_state(p.drop, seed, offset);
+    if (drop) drop_state(p.drop, seed, offset);
+    const KeysAdded added{(uint32_t)seed, (uint32_t)(seed >> 32)};
+    if (threadIdx.x < 10) {                              // registers are what this kernel is short of
+        keys_[2 * threadIdx.x] = added.at(threadIdx.x).x;
+        keys_[2 * threadIdx.x + 1] = added.at(threadIdx.x).y;
+    }
+    const KeysShared keys{smem_u32(keys_)};
     if (blockIdx.x == 0 && threadIdx.x == 0 && p.counter) *p.counter = 0;    // block_param_kernel counts its CTAs here
     float2 colA[RES ? FR : 1][P], colB[FR][P];
 #pragma unroll
@@ -352,7 +383,7 @@ __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && si
     for (; tok < p.n_tok; tok += step, stage ^= 1) {
         const long long row = tok * p.d + own;           // this lane's first element of the row
         const float ry = RES && w ? p.r_y[tok] : 1.f;
-        const float ro = du ? p.r_o[tok] : 0.f;
+        const float ro = has_u ? p.r_o[tok] : 0.f;
         const float gt = RES && p.gate_kind == kGateToken ? S::load1(static_cast<const T *>(p.gate) + tok) : 1.f;
         const float2 ry2 = splat(ry), ro2 = splat(ro);
         cp_async_wait<1>();
@@ -378,18 +409,18 @@ __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && si
 #pragma unroll
                         for (int i = 0; i < P; ++i) b[i] = __fmul2_rn(b[i], c[i]);
                     }
-                    if (p.drop.threshold) {
-                        drop_words<P>(words[k], (unsigned long long)(row + k * 32 * VEC), seed, offset);
+                    if (drop) {
+                        drop_words<P>(words[k], (unsigned long long)(row + k * 32 * VEC), keys, offset);
                         drop_pairs<P>(b, words[k], p.drop.threshold);
                     }
-                    if (dout) {
+                    if (has_out) {
                         S::unpack2(lds_v4(slot(stage, 3, k)), c);
 #pragma unroll
                         for (int i = 0; i < P; ++i) s2 = __ffma2_rn(b[i], c[i], s2);
                     }
                 }
             }
-            if (in && du) {
+            if (in && has_u) {
                 float2 uu[P];
                 S::unpack2(lds_v4(slot(stage, 1, k)), oh[k]);
                 S::unpack2(lds_v4(slot(stage, 0, k)), uu);
@@ -427,14 +458,14 @@ __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && si
             for (int k = 0; k < FR; ++k) {
                 if (f0 + 32 * k >= p.frags) continue;
                 float2 v[P], yh[P];
-                if (dout) S::unpack2(lds_v4(slot(stage, 3, k)), v);
+                if (has_out) S::unpack2(lds_v4(slot(stage, 3, k)), v);
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
                     D[k][i] = __ffma2_rn(c1, oh[k][i], D[k][i]);
-                    D[k][i] = dout ? __ffma2_rn(ro2, D[k][i], v[i]) : __fmul2_rn(ro2, D[k][i]);
+                    D[k][i] = has_out ? __ffma2_rn(ro2, D[k][i], v[i]) : __fmul2_rn(ro2, D[k][i]);
                 }
                 if (dx) st_global_v4(dx + row + k * 32 * VEC, S::pack2v(D[k]));
-                if (p.drop.threshold) drop_pairs<P>(D[k], words[k], p.drop.threshold);
+                if (drop) drop_pairs<P>(D[k], words[k], p.drop.threshold);
                 S::unpack2(lds_v4(slot(stage, 2, k)), yh);
 #pragma unroll
                 for (int i = 0; i < P; ++i) yh[i] = __fmul2_rn(yh[i], ry2);
@@ -462,6 +493,7 @@ __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && si
         }
     }
     if (!p.part) return;
+    grid_launch_dependents();                            // block_param_kernel's CTAs may come up as these leave
     float *mine = p.part + (long long)blockIdx.x * 2 * p.d;
     float *cols = reinterpret_cast<float *>(dyn);        // [2][d]
     cp_async_wait<0>();
@@ -497,6 +529,7 @@ __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && si
 template <typename W>
 __global__ void __launch_bounds__(1024) block_param_kernel(const BlockParams p, int rows) {
     __shared__ double sa[32][33], sb[32][33];
+    grid_wait();
     const int c = threadIdx.x & 31, r0 = threadIdx.x >> 5;
     const int col = blockIdx.x * 32 + c;
     double a = 0., b = 0.;
@@ -554,14 +587,19 @@ __global__ void __launch_bounds__(1024) block_param_kernel(const BlockParams p, 
 
 // out = m x over n elements in row-major order: forward, and backward with the gradient as x
 template <typename T>
-__global__ void __launch_bounds__(256) dropout_kernel(const T *__restrict__ x, T *__restrict__ out, long long n, DropParams dp) {
+// (four CTAs per SM with two fragments in flight per thread: 25 us for 32768 x 1024 bf16; three with four 29)
+__global__ void __launch_bounds__(256, 4) dropout_kernel(const T *__restrict__ x, T *__restrict__ out, long long n, DropParams dp) {
     using S = Store<T>;
     constexpr int VEC = S::kVec;
     unsigned long long seed, offset;
     drop_state(dp, seed, offset);
-    if (dp.rng_used && blockIdx.x == 0 && threadIdx.x == 0) {
-        dp.rng_used[0] = (long long)seed;
-        dp.rng_used[1] = (long long)offset;
+    const KeysAdded added{(uint32_t)seed, (uint32_t)(seed >> 32)};
+    KeysHeld keys;
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        keys.k0[r] = added.at(r).x;
+        keys.k1[r] = added.at(r).y;
+        asm volatile("" : "+r"(keys.k0[r]), "+r"(keys.k1[r]));   // held, not added up again at every use
     }
     constexpr int P = S::kPairs;
     const long long frags = n / VEC, stride = (long long)gridDim.x * blockDim.x;
@@ -570,24 +608,22 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T *__restrict__ x, T
         float2 v[P];
         uint32_t words[P];
         S::unpack2(q, v);
-        drop_words<P>(words, (unsigned long long)(f * VEC), seed, offset);
+        drop_words<P>(words, (unsigned long long)(f * VEC), keys, offset);
 #pragma unroll
         for (int i = 0; i < P; ++i) v[i] = __fmul2_rn(v[i], scale);
         drop_pairs<P>(v, words, dp.threshold);
         return S::pack2v(v);
     };
     long long f = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    for (; f + 3 * stride < frags; f += 4 * stride) {    // four fragments in flight
-        uint4 q[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = ld_global_stream_v4(x + (f + i * stride) * VEC);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) st_global_v4(out + (f + i * stride) * VEC, masked(q[i], f + i * stride));
+    for (; f + stride < frags; f += 2 * stride) {
+        const uint4 q0 = ld_global_stream_v4(x + f * VEC), q1 = ld_global_stream_v4(x + (f + stride) * VEC);
+        st_global_v4(out + f * VEC, masked(q0, f));
+        st_global_v4(out + (f + stride) * VEC, masked(q1, f + stride));
     }
     for (; f < frags; f += stride) st_global_v4(out + f * VEC, masked(ld_global_stream_v4(x + f * VEC), f));
     if (f == frags && frags * VEC < n) {                 // the elements behind the last whole fragment: one thread
         uint32_t words[P];
-        drop_words<P>(words, (unsigned long long)(frags * VEC), seed, offset);
+        drop_words<P>(words, (unsigned long long)(frags * VEC), keys, offset);
         for (int e = 0; frags * VEC + e < n; ++e) {
             const uint32_t h = e & 1 ? words[e >> 1] >> 16 : words[e >> 1] & 0xffffu;
             S::store1(out + frags * VEC + e, h >= dp.threshold ? S::load1(x + frags * VEC + e) * dp.keep_scale : 0.f);
@@ -612,15 +648,15 @@ static bool block_shape(int frags, long long n_tok, int sms, int most, int *fr, 
 }
 
 // CTAs of 256 threads an SM holds, by registers (of 65,536, in units of 256 per warp) and shared memory
-static int registers_of(const void *kernel) {
+static int registers_of(void (*kernel)(const BlockParams)) {
     cudaFuncAttributes at;
-    if (cudaFuncGetAttributes(&at, kernel) == cudaSuccess) return at.numRegs;
+    if (cudaFuncGetAttributes(&at, reinterpret_cast<const void *>(kernel)) == cudaSuccess) return at.numRegs;
     cudaGetLastError();
     return 255;
 }
 static int resident(int regs, size_t smem) {
     const int by_regs = 65536 / (kBlkWarps * ((regs * 32 + 255) / 256 * 256));
-    const int by_smem = (int)((size_t)(228 * 1024) / (smem + 256 + 1024));
+    const int by_smem = (int)((size_t)(228 * 1024) / (smem + 384 + 1024));
     const int n = by_regs < by_smem ? by_regs : by_smem;
     return n < 1 ? 1 : n > 8 ? 8 : n;
 }
@@ -644,16 +680,23 @@ static cudaError_t launch_block_t(BlockParams p, bool bwd, int sms, cudaStream_t
     size_t smem = ring_bytes(arrays, fr) + sizeof(float) * (RES ? 2 : 1) * p.frags * Store<T>::kVec;
     if (bwd && smem < sizeof(float) * 2 * p.d) smem = sizeof(float) * 2 * p.d;
     const long long need = (p.n_tok + groups - 1) / groups;
+    using Kernel = void (*)(const BlockParams);
+    // the form (see the kernels) and its registers per thread, looked up once
+    const int form = !RES ? 0 : bwd ? (full || !p.d_u || !p.d_out ? 0 : p.drop.threshold ? 2 : 1) : !full && !p.drop.threshold;
 #define LB_BLK(FR_)                                                                                                  \
     case FR_: {                                                                                                      \
-        auto kernel = bwd ? block_bwd_kernel<T, W, FR_, RES> : block_fwd_kernel<T, W, FR_, RES>;                     \
-        cudaError_t e = cudaSuccess;                                                                                 \
-        if (smem > 40 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
-        if (e != cudaSuccess) return e;                                                                              \
-        static const int regs[2] = {registers_of(reinterpret_cast<const void *>(block_fwd_kernel<T, W, FR_, RES>)),  \
-                                    registers_of(reinterpret_cast<const void *>(block_bwd_kernel<T, W, FR_, RES>))}; \
-        const int per_sm = resident(regs[bwd], smem);                                                                \
-        long long cap = (long long)sms * per_sm;                                                                     \
+        static const Kernel kernels[5] = {block_fwd_kernel<T, W, FR_, RES, 0>, block_fwd_kernel<T, W, FR_, RES, RES ? 1 : 0>, \
+                                          block_bwd_kernel<T, W, FR_, RES, 0>, block_bwd_kernel<T, W, FR_, RES, RES ? 1 : 0>, \
+                                          block_bwd_kernel<T, W, FR_, RES, RES ? 2 : 0>};                            \
+        static const int regs[5] = {registers_of(kernels[0]), registers_of(kernels[1]), registers_of(kernels[2]),    \
+                                    registers_of(kernels[3]), registers_of(kernels[4])};                             \
+        const int which = (bwd ? 2 : 0) + form;                                                                      \
+        const Kernel kernel = kernels[which];                                                                        \
+        if (smem > 40 * 1024) {                                                                                      \
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
+            if (e != cudaSuccess) return e;                                                                          \
+        }                                                                                                            \
+        long long cap = (long long)sms * resident(regs[which], smem);                                                \
         if (bwd && cap > block_bwd_rows(sms)) cap = block_bwd_rows(sms);                                             \
         grid = (int)(need < cap ? need : cap);                                                                       \
         kernel<<<grid, kBlkThreads, smem, stream>>>(p);                                                              \
@@ -666,8 +709,7 @@ static cudaError_t launch_block_t(BlockParams p, bool bwd, int sms, cudaStream_t
 #undef LB_BLK
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || !bwd || !p.part) return e;
-    block_param_kernel<W><<<(p.d + 31) / 32, 1024, 0, stream>>>(p, grid);
-    return cudaGetLastError();
+    return launch_after(block_param_kernel<W>, dim3((p.d + 31) / 32), dim3(1024), 0, stream, 1, true, p, grid);
 }
 
 int block_bwd_rows(int sms) { return 2 * sms < 304 ? 2 * sms : 304; }

@@ -1,6 +1,7 @@
 // The gated feed-forward block's launches: which instantiation of the matrix product, and the sum of its slices along k.
 #include "lb_common.cuh"
 #include "lb_kernels.h"
+#include "lb_launch.cuh"
 
 namespace lb {
 
@@ -20,6 +21,8 @@ cudaError_t launch_gemm(int tile, int epilogue, int form, const GemmMaps &maps, 
 __global__ void __launch_bounds__(256) gemm_sum_kernel(const float *__restrict__ part, __nv_bfloat16 *__restrict__ out, int splits,
                                                        long long n) {
     const long long stride = (long long)gridDim.x * blockDim.x;
+    grid_wait();
+    grid_launch_dependents();
     for (long long f = (long long)blockIdx.x * blockDim.x + threadIdx.x; f < n / 8; f += stride) {
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         for (int s = 0; s < splits; ++s) {
@@ -33,8 +36,8 @@ __global__ void __launch_bounds__(256) gemm_sum_kernel(const float *__restrict__
 
 cudaError_t launch_gemm_sum(const float *part, void *out, int splits, long long n, int sms, cudaStream_t stream) {
     const long long need = (n / 8 + 255) / 256, cap = 16LL * sms;
-    gemm_sum_kernel<<<(int)(need < cap ? need : cap), 256, 0, stream>>>(part, static_cast<__nv_bfloat16 *>(out), splits, n);
-    return cudaGetLastError();
+    return launch_after(gemm_sum_kernel, dim3((unsigned)(need < cap ? need : cap)), dim3(256), 0, stream, 1, true, part,
+                        static_cast<__nv_bfloat16 *>(out), splits, n);
 }
 
 }  // namespace lb

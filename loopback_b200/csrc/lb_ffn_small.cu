@@ -60,8 +60,8 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(const __grid_c
     const uint32_t tmem = (uint32_t)lds_volatile_s32(slot);
     if (warp == 0) {
         if (lane == 0) {
-            if constexpr (GATED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-            else asm volatile("griddepcontrol.wait;" ::: "memory");                                  // h is complete
+            if constexpr (GATED) grid_launch_dependents();
+            else grid_wait();                            // h is complete
             for (int i = 0; i < ahead; ++i) tokens(i, kb0 + i);
             int s = 0;
             uint32_t ph = 1;
@@ -187,27 +187,7 @@ static cudaError_t launch_small_t(const CUtensorMap &w0, const CUtensorMap &w1, 
     auto kernel = ffn_small_kernel<N, GATED>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmMaxSmem);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * split));
-    cfg.blockDim = dim3(kSmallThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute at[2];
-    int n = 0;
-    if (split > 1) {
-        at[n].id = cudaLaunchAttributeClusterDimension;
-        at[n].val.clusterDim.x = split;
-        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
-        ++n;
-    }
-    if (!GATED) {
-        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[n].val.programmaticStreamSerializationAllowed = 1;
-        ++n;
-    }
-    cfg.attrs = at;
-    cfg.numAttrs = n;
-    return cudaLaunchKernelEx(&cfg, kernel, w0, w1, x, p);
+    return launch_after(kernel, dim3((unsigned)(tiles * split)), dim3(kSmallThreads), smem, stream, split, !GATED, w0, w1, x, p);
 }
 
 cudaError_t launch_ffn_small(bool gated, int rows, const CUtensorMap &w0, const CUtensorMap &w1, const CUtensorMap &x,

@@ -14,6 +14,7 @@
 
 #include "lb_common.cuh"
 #include "lb_kernels.h"
+#include "lb_launch.cuh"
 
 namespace lb {
 
@@ -263,6 +264,8 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
     else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = (uint32_t)lds_volatile_s32(slot);
+    grid_wait();
+    grid_launch_dependents();
 
     const int tiles = p.m_tiles * p.n_tiles * p.splits + p.m_tiles2 * p.n_tiles2;
     const int first = blockIdx.x / CG, step = gridDim.x / CG;
@@ -544,18 +547,8 @@ cudaError_t launch_gemm_t(const GemmMaps &maps, const GemmParams &p, int sms, cu
     const long long tiles = (long long)p.m_tiles * p.n_tiles * p.splits + (long long)p.m_tiles2 * p.n_tiles2;
     const long long groups = sms / CG;
     if (tiles < 1 || tiles + groups > 0x7fffffffLL) return cudaErrorInvalidValue;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(CG * (tiles < groups ? tiles : groups)));
-    cfg.blockDim = dim3(Sh::kThreads);
-    cfg.dynamicSmemBytes = Sh::kSmem;
-    cfg.stream = stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = CG;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = CG == 2 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, maps, p);
+    return launch_after(kernel, dim3((unsigned)(CG * (tiles < groups ? tiles : groups))), dim3(Sh::kThreads), Sh::kSmem, stream, CG,
+                        p.after != 0, maps, p);
 }
 
 }  // namespace lb

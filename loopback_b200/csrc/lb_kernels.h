@@ -240,6 +240,7 @@ struct GemmParams {
     int m_tiles, n_tiles, splits;
     int m2, n2, m_tiles2, n_tiles2;   // kFormMN: a second product over the same k in the same launch (m_tiles2 = 0: none)
     int act;                  // LB_ACT_*
+    int after;                // launched behind another kernel of the same call (see lb_launch.cuh)
     uint8_t *kept;            // act'(g) u and act(g) in blocks of 32 x 32 (kEpiGate: null = not kept)
     int *err_word;
     long long wait_cycles;

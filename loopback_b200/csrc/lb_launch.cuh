@@ -1,0 +1,38 @@
+// Launches that follow one another on a stream: a kernel launched `after` its predecessor may have its CTAs set up while the
+// predecessor's last ones run (programmatic stream serialisation). Such a kernel calls grid_wait() before it touches anything
+// another kernel wrote or reads: that waits for the predecessor's end, its memory included.
+#pragma once
+
+#include <cuda_runtime.h>
+
+namespace lb {
+
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename Kernel, typename... Args>
+cudaError_t launch_after(Kernel kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, int cluster, bool after, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[2];
+    int n = 0;
+    if (cluster > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = cluster;
+        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (after) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+}  // namespace lb
