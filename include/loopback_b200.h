@@ -67,7 +67,7 @@ int lb_device_error(int clear);
  * gradients takes the kernels for few rows; -1 never), "block_frags" (16-byte fragments of a row per lane of the
  * norm and residual kernels at most: 1..4), "wait_cycles" (the limit of
  * every bounded wait inside the kernels, in GPU clock cycles; default 4e9), "test_skip_item" (test hook: the first
- * CTA of the next forward reads leaves out its k-th tile copy, so that a bounded wait runs out, the CTA unwinds and
+ * CTA of the next forward reads and feed-forward products leaves out its k-th tile copy, so that a bounded wait runs out, the CTA unwinds and
  * lb_device_error reports it; nothing traps or hangs). Value 0 restores the default
  * (chosen by size); the name "reset_all" restores every knob. Returns LB_ERR_ARG for an unknown name.
  * The knobs are one process-wide table without a lock: set them from one thread, while no other thread is inside

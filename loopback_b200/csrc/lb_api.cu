@@ -965,7 +965,7 @@ static int run_gemm(const char *who, int epi, int form, const GemmPlan &pl, cons
     }
     p.m = (int)m; p.n = (int)n; p.kblocks = (int)((k + 63) / 64); p.segs = segs;
     p.m_tiles = pl.m_tiles; p.n_tiles = pl.n_tiles; p.splits = pl.splits; p.m_tiles2 = pl.m_tiles2; p.n_tiles2 = pl.n_tiles2;
-    p.m2 = two ? (int)c[1].rows : 0; p.n2 = two ? (int)c[1].cols : 0; p.act = act; p.after = after; p.kept = static_cast<uint8_t *>(kept);
+    p.m2 = two ? (int)c[1].rows : 0; p.n2 = two ? (int)c[1].cols : 0; p.act = act; p.after = after; p.test_skip_item = g_opt.test_skip_item; p.kept = static_cast<uint8_t *>(kept);
     p.err_word = di.err_word; p.wait_cycles = wait_limit();
     cudaError_t err = lb::launch_gemm(pl.tile, split ? (int)lb::kEpiPartial : epi, form, maps, p, di.sms, st);
     if (err == cudaSuccess && split)
@@ -1069,6 +1069,7 @@ int lb_ffn_fwd(const void *x, const void *w_gate, const void *w_up, const void *
         CUtensorMap m0, m1, mx;
         lb::FfnSmallParams p;
         p.n_tok = (int)n_tok; p.act = act; p.err_word = di.err_word; p.wait_cycles = wait_limit();
+        p.test_skip_item = g_opt.test_skip_item;
         if ((rc = make_map_tile(&m0, w_gate, f, d, d, 64)) || (rc = make_map_tile(&m1, w_up, f, d, d, 64)) ||
             (rc = make_map_tile(&mx, x, n_tok, d, d, rows))) return rc;
         p.out = h; p.n = f; p.kblocks = (d + 63) / 64;

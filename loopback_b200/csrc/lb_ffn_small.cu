@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(const __grid_c
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     const int ST = p.stages;
     const uint32_t bars = base + ST * kStage;
-    const uint32_t full = bars, empty = full + 8 * ST, done = empty + 8 * ST, slot = done + 8, abort_flag = slot + 4;
+    const uint32_t full = bars, empty = full + 8 * ST, done = empty + 8 * ST, mdone = done + 8, slot = mdone + 8, abort_flag = slot + 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = p.split > 1 ? cluster_rank() : 0;
     const int tile = blockIdx.x / p.split;
@@ -38,6 +38,7 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(const __grid_c
     const auto weights = [&](int s, int kb) {
         const uint32_t sa = base + s * kStage, bar = full + 8 * s;
         mbar_arrive_expect_tx(bar, kStage);
+        if (p.test_skip_item != 0 && blockIdx.x == 0 && kb + 1 == p.test_skip_item) return;      // test hook: never comes
         tma_load_2d(sa, &map_w0, bar, kb * kGemmK, row0);
         if constexpr (GATED) tma_load_2d(sa + kA / 2, &map_w1, bar, kb * kGemmK, row0);
     };
@@ -48,6 +49,7 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(const __grid_c
             mbar_init(empty + 8 * i, 1);
         }
         mbar_init(done, 1);
+        mbar_init(mdone, 1);
         sts_s32(abort_flag, 0);
         fence_mbar_init();
         for (int i = 0; i < ahead; ++i) weights(i, kb0 + i);     // before anything else of the CTA is ready
@@ -97,6 +99,7 @@ __global__ void __launch_bounds__(kSmallThreads) ffn_small_kernel(const __grid_c
                 if (++s == ST) { s = 0; ph ^= 1; }
             }
             if (ok) tc_commit<1>(done);
+            tc_drain<1>(mdone, p.wait_cycles);
         }
     } else if (warp_wait(done, 0, wc, kDevWaitTmem)) {
         // this CTA's sums, [token][128 weight rows] fp32, over the ring (all its tiles have been read)

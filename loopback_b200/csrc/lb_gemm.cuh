@@ -121,6 +121,13 @@ template <int CG> __device__ __forceinline__ void tc_commit(uint32_t bar) {
         asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                      ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
+// Waits, with a limit, until every multiply issued has been done: shared memory and TMEM may not go away under one, whoever
+// gave up a wait before.
+template <int CG> __device__ __forceinline__ void tc_drain(uint32_t bar, long long limit) {
+    tc_commit<CG>(bar);
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, 0) && clock64() - t0 < limit) {}
+}
 // 32 accumulator columns of this thread's row
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
     uint32_t *r = reinterpret_cast<uint32_t *>(v);
@@ -239,8 +246,8 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     const uint32_t staging = base + ST * Sh::kStageBytes;
     const uint32_t bars = staging + Sh::kStaging;
-    const uint32_t full = bars, empty = full + 8 * ST, tfull = empty + 8 * ST, tempty = tfull + 16, slot = tempty + 16,
-                   abort_flag = slot + 4;
+    const uint32_t full = bars, empty = full + 8 * ST, tfull = empty + 8 * ST, tempty = tfull + 16, mdone = tempty + 16,
+                   slot = mdone + 8, abort_flag = slot + 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0;
     WaitCtx wc{abort_flag, p.err_word, p.wait_cycles};
@@ -254,6 +261,7 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
             mbar_init(tfull + 8 * i, 1);
             mbar_init(tempty + 8 * i, CG * EW);
         }
+        mbar_init(mdone, 1);
         sts_s32(abort_flag, 0);
         fence_mbar_init();
     }
@@ -289,7 +297,9 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
                     const int seg = A_MN ? at.product : half;
                     const uint32_t sa = base + s * Sh::kStageBytes, sb = sa + Sh::kABytes, bar = lead_full + 8 * s;
                     if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, CG * Sh::kStageBytes);
-                    if constexpr (!A_MN) {
+                    if (p.test_skip_item != 0 && blockIdx.x == 0 && issued + 1 == p.test_skip_item) {
+                        // test hook: this copy never comes
+                    } else if constexpr (!A_MN) {
                         tma_tile<CG>(sa, &maps.a[seg], bar, k0, m0);
                     } else {
 #pragma unroll
@@ -354,6 +364,7 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
                 tc_commit<CG>(tfull + 8 * acc);
                 if (++acc == 2) { acc = 0; aph ^= 1; }
             }
+            tc_drain<CG>(mdone, p.wait_cycles);
         }
     } else {
         const int ew = warp - 2, quad = warp & 3, half = ew >> 2;

@@ -241,6 +241,7 @@ struct GemmParams {
     int m2, n2, m_tiles2, n_tiles2;   // kFormMN: a second product over the same k in the same launch (m_tiles2 = 0: none)
     int act;                  // LB_ACT_*
     int after;                // launched behind another kernel of the same call (see lb_launch.cuh)
+    int test_skip_item;       // test hook: the first CTA's k-th copy of A is left out (0 = off)
     uint8_t *kept;            // act'(g) u and act(g) in blocks of 32 x 32 (kEpiGate: null = not kept)
     int *err_word;
     long long wait_cycles;
@@ -267,6 +268,7 @@ struct FfnSmallParams {
     int n_tok, n;             // n: columns of the result (= weight rows of one projection)
     int kblocks;              // blocks of 64 along k
     int act;
+    int test_skip_item;       // test hook: the first CTA's copy of the k-th block of weights is left out (0 = off)
     int split = 1, stages = 1;   // CTAs per tile, ring depth (filled in by the launcher)
     int *err_word;
     long long wait_cycles;

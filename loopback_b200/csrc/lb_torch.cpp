@@ -74,6 +74,12 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
     return false;
 }
 
+// contiguous and on a 16-byte boundary (a view may begin anywhere), a copy where it is not
+Tensor dense(const Tensor &t) {
+    Tensor c = t.contiguous();
+    return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15) ? c.clone() : c;
+}
+
 Tensor bytes(size_t n, const Tensor &like) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
 Tensor floats(int64_t n, const Tensor &like) { return at::empty({n}, like.options().dtype(at::kFloat)); }
 
@@ -93,7 +99,7 @@ void channel_params(const Tensor &x, std::initializer_list<Tensor *> ps, const c
         seen = true;
     }
     for (Tensor *p : ps)
-        if (p->defined()) *p = (cast ? p->to(at::kFloat) : *p).contiguous();
+        if (p->defined()) *p = dense(cast ? p->to(at::kFloat) : *p);
 }
 
 // Under create_graph the results of a backward would be taken for constants: they raise where somebody differentiates them.
@@ -129,7 +135,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
         const variable_list s = ctx->get_saved_variables();
         const Tensor &x = s[0], &w = s[1], &r = s[2];
         const int64_t d = x.size(-1);
-        const Tensor du = g[0].contiguous();
+        const Tensor du = dense(g[0]);
         Tensor dx, dw, scratch;
         if (ctx->needs_input_grad(0)) dx = at::empty_like(x);
         if (ctx->needs_input_grad(1)) {
@@ -146,7 +152,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
 Tensor block_norm(const Tensor &x, Tensor w, double eps) {
     require_rows(x, "block_norm");
     channel_params(x, {&w}, "block_norm");
-    const Tensor xc = x.contiguous();
+    const Tensor xc = dense(x);
     return wants_grad({xc, w}) ? BlockNorm::apply(xc, w, eps) : norm_forward(xc, w, eps, nullptr);
 }
 
@@ -181,7 +187,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list g) {
         const Tensor used = ctx->get_saved_variables()[0];
-        Tensor dx = dropout_launch(g[0].contiguous(), ctx->saved_data["threshold"].toInt(), used, ctx->saved_data["seed"].toInt(),
+        Tensor dx = dropout_launch(dense(g[0]), ctx->saved_data["threshold"].toInt(), used, ctx->saved_data["seed"].toInt(),
                                    ctx->saved_data["offset"].toInt(), Tensor());
         return once({dx, Tensor(), Tensor(), Tensor(), Tensor()}, "dropout");
     }
@@ -191,7 +197,7 @@ Tensor dropout(const Tensor &x, int64_t threshold, const Maybe &rng, int64_t see
     TORCH_CHECK(x.is_cuda(), "loopback_b200.dropout: tensors must live on a CUDA device (there is no CPU path)");
     const Tensor pair = rng.value_or(Tensor());
     check_rng(x, pair, "dropout");
-    const Tensor xc = x.contiguous();
+    const Tensor xc = dense(x);
     return wants_grad({xc}) ? Dropout::apply(xc, rng, threshold, seed, offset)
                             : dropout_launch(xc, threshold, pair, seed, offset, Tensor());
 }
@@ -247,8 +253,8 @@ struct BlockResidual : torch::autograd::Function<BlockResidual> {
     static variable_list backward(AutogradContext *ctx, variable_list g) {
         const variable_list s = ctx->get_saved_variables();
         const Tensor &x = s[0], &y = s[1], &w = s[2], &gate = s[3], &scale = s[4], &next_w = s[5], &stats = s[6];
-        const Tensor g_out = g[0].defined() ? g[0].contiguous() : Tensor();
-        const Tensor g_u = g.size() > 1 && g[1].defined() ? g[1].contiguous() : Tensor();
+        const Tensor g_out = g[0].defined() ? dense(g[0]) : Tensor();
+        const Tensor g_u = g.size() > 1 && g[1].defined() ? dense(g[1]) : Tensor();
         if (!g_out.defined() && !g_u.defined()) return variable_list(8);
         const int kind = (int)ctx->saved_data["kind"].toInt();
         const int64_t d = x.size(-1), n = x.numel() / d;
@@ -296,7 +302,7 @@ variable_list block_residual(const Tensor &x, const Tensor &y, const Maybe &weig
                     "loopback_b200.block_residual: a gate per token or element has the rows' type, got ", gate.scalar_type());
     }
     channel_params(x, {&w, &next_w, a.kind == LB_GATE_CHANNEL ? &gate : &none}, what);
-    if (gate.defined()) gate = gate.contiguous();
+    if (gate.defined()) gate = dense(gate);
     if (scale_t.defined()) {
         TORCH_CHECK(scale_t.numel() == 1, "loopback_b200.block_residual: a learned scale has one element");
         same_device(x, scale_t, what);
@@ -304,7 +310,7 @@ variable_list block_residual(const Tensor &x, const Tensor &y, const Maybe &weig
     }
     check_rng(x, rng, what);
     a.scale = scale; a.eps = eps; a.threshold = threshold; a.seed = seed; a.offset = offset;
-    const Tensor xc = x.contiguous(), yc = y.contiguous();
+    const Tensor xc = dense(x), yc = dense(y);
     if (wants_grad({xc, yc, w, gate, scale_t, next_w})) {
         const auto maybe = [](const Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); };
         return BlockResidual::apply(xc, yc, maybe(w), maybe(gate), maybe(scale_t), maybe(next_w), maybe(rng), &a);
@@ -344,7 +350,7 @@ struct GatedFFN : torch::autograd::Function<GatedFFN> {
         const variable_list s = ctx->get_saved_variables();
         const Tensor &x = s[0], &wg = s[1], &wu = s[2], &wd = s[3], &h = s[4], &kept = s[5];
         const int64_t d = x.size(-1), f = wg.size(0), n = x.numel() / d;
-        const Tensor dy = g[0].contiguous();
+        const Tensor dy = dense(g[0]);
         const bool need_g = ctx->needs_input_grad(1), need_u = ctx->needs_input_grad(2);
         Tensor dx, dgu, dwd;
         if (ctx->needs_input_grad(0)) dx = at::empty_like(x);
@@ -370,7 +376,7 @@ Tensor gated_ffn(const Tensor &x, const Tensor &wg, const Tensor &wu, const Tens
         TORCH_CHECK(t->scalar_type() == at::kBFloat16, "loopback_b200.gated_ffn: the products run in bf16, got ", t->scalar_type());
     for (const Tensor *w : {&wg, &wu, &wd}) TORCH_CHECK(w->is_contiguous(), "loopback_b200.gated_ffn: weights must be contiguous");
     TORCH_CHECK(d < (1 << 30) && wg.size(0) < (1 << 30), "loopback_b200.gated_ffn: d=", d, ", f=", wg.size(0), " are too large");
-    const Tensor xc = x.contiguous();
+    const Tensor xc = dense(x);
     return wants_grad({xc, wg, wu, wd}) ? GatedFFN::apply(xc, wg, wu, wd, act) : ffn_forward(xc, wg, wu, wd, act, Tensor(), Tensor());
 }
 

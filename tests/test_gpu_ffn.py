@@ -173,9 +173,16 @@ def test_shapes_frozen_weights_and_empty_batches():
         ins = [v.detach().requires_grad_(i == j) for j, v in enumerate((x, wg, wu, wd))]
         (g,) = torch.autograd.grad(block.gated_ffn(*ins), ins[i], dy)
         assert torch.equal(g, full[i])
+    odd = torch.empty(60 * 72 + 3, device="cuda", dtype=torch.bfloat16)[3:].view(60, 72).copy_(x.detach())   # not on 16 bytes
+    assert torch.equal(block.gated_ffn(odd, wg.detach(), wu.detach(), wd.detach()), y)
     fused = torch.cat((wg, wu)).detach()                  # one parameter holding both projections
     assert torch.equal(block.gated_ffn(x.detach(), *fused.chunk(2), wd.detach()), y)
     e = torch.zeros(0, 72, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    same = wg.detach().requires_grad_()                   # one tensor as both projections: its two gradients add up
+    xs = x.detach()
+    (gs,) = torch.autograd.grad(block.gated_ffn(xs, same, same, wd), same, dy)
+    w1, w2 = (wg.detach().clone().requires_grad_() for _ in range(2))
+    assert torch.equal(gs, sum(torch.autograd.grad(block.gated_ffn(xs, w1, w2, wd), (w1, w2), dy)))
     ge = torch.autograd.grad(block.gated_ffn(e, wg, wu, wd), (e, wg, wu, wd), torch.zeros_like(e))
     assert ge[0].shape == e.shape and not any(g.any() for g in ge[1:])
 
@@ -206,6 +213,32 @@ def test_on_another_stream_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(grads, want))
 
 
+@pytest.mark.parametrize("t,tile", [(300, 1), (300, 3), (40, 0)])
+def test_a_wait_that_runs_out_unwinds_and_reports(t, tile):
+    """The products' waits are bounded. With the limit at about a millisecond and the hook that leaves out one tile copy of the
+    first CTA, its multiplies give up, everybody unwinds, the kernel returns and the device error word names a wait; the next
+    launch is unaffected."""
+    import loopback_b200._lib as L
+    from loopback_b200 import block
+    (x, wg, wu, wd), _ = _inputs(t, 264, 520, 4, grad=False)
+    try:
+        L.set_option("ffn_tile", tile)
+        good = block.gated_ffn(x, wg, wu, wd)
+        assert L.device_error() == 0
+        L.set_option("wait_cycles", 2_000_000)
+        L.set_option("test_skip_item", 2)
+        block.gated_ffn(x, wg, wu, wd)
+        torch.cuda.synchronize()
+        L.set_option("wait_cycles", 0)
+        L.set_option("test_skip_item", 0)
+        # the first wait to run out: for a tile, a free stage, the producer's last stages (begun as early, with a tile this
+        # short), an accumulator
+        assert L.device_error(clear=True) in (1, 2, 5, 7)
+        assert torch.equal(block.gated_ffn(x, wg, wu, wd), good) and L.device_error() == 0
+    finally:
+        L.reset_options()
+
+
 def test_two_calls_at_once():
     """Two streams at the same time: each call has a workspace of its own."""
     from loopback_b200 import block
@@ -231,7 +264,7 @@ def test_refusals():
                  lambda: block.gated_ffn(x, wg, wu, wd.t().contiguous()), lambda: block.gated_ffn(x, wg, wu[:64], wd),
                  lambda: block.gated_ffn(x, wg.t().contiguous().t(), wu, wd), lambda: block.gated_ffn(x, wg.cpu(), wu, wd),
                  lambda: block.gated_ffn(x[:, :36].contiguous(), wg[:, :36].contiguous(), wu[:, :36].contiguous(), wd[:36]),
-                 lambda: block.gated_ffn(x.view(-1)[4:4 + 64 * 7].view(7, 64), wg, wu, wd),
+                 lambda: block.gated_ffn(x, wg.view(-1)[4:4 + 64 * 64].view(64, 64), wu[:64], wd[:, :64].contiguous()),
                  lambda: block.gated_ffn(wide[:, :0], wide[:0], wide[:0], wide[:0])):
         with pytest.raises(RuntimeError):
             call()
