@@ -324,7 +324,7 @@ size_t lb_ffn_workspace_bytes(int64_t n_tok, int d, int f, int kind);
  * act(g) with 24 bits each, 6 bytes per element of h, rows and columns rounded up to 32). */
 size_t lb_ffn_kept_bytes(int64_t n_tok, int f);
 
-/* Training: h [n_tok][f] and kept are written for the backward. Inference: both NULL, and up to 128 rows (a decode step) take
+/* Training: h [n_tok][f] and kept are written for the backward. Inference: both NULL, and up to 64 rows (a decode step) take
  * kernels of their own, bound by reading the weights once. */
 int lb_ffn_fwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, void *y, void *h, void *kept,
                void *workspace, size_t workspace_bytes, int64_t n_tok, int d, int f, int act, int dtype, void *stream);

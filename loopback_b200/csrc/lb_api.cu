@@ -942,7 +942,7 @@ struct Operand {
 // One product m x n over `segs` segments of k columns each, c[0] (through `part` where k is split); or, where the plan says so,
 // two products over the same k: a[0] b[0] -> c[0] and a[1] b[1] -> c[1].
 static int run_gemm(const char *who, int epi, int form, const GemmPlan &pl, const Operand *a, const Operand *b, const Operand *c,
-                    void *kept, void *part, long long m, long long n, long long k, int segs, int act, bool after,
+                    void *kept, void *part, long long m, long long n, long long k, int segs, int act,
                     const DeviceInfo &di, cudaStream_t st) {
     lb::GemmMaps maps;
     memset(&maps, 0, sizeof maps);
@@ -965,7 +965,7 @@ static int run_gemm(const char *who, int epi, int form, const GemmPlan &pl, cons
     }
     p.m = (int)m; p.n = (int)n; p.kblocks = (int)((k + 63) / 64); p.segs = segs;
     p.m_tiles = pl.m_tiles; p.n_tiles = pl.n_tiles; p.splits = pl.splits; p.m_tiles2 = pl.m_tiles2; p.n_tiles2 = pl.n_tiles2;
-    p.m2 = two ? (int)c[1].rows : 0; p.n2 = two ? (int)c[1].cols : 0; p.act = act; p.after = after; p.test_skip_item = g_opt.test_skip_item; p.kept = static_cast<uint8_t *>(kept);
+    p.m2 = two ? (int)c[1].rows : 0; p.n2 = two ? (int)c[1].cols : 0; p.act = act; p.test_skip_item = g_opt.test_skip_item; p.kept = static_cast<uint8_t *>(kept);
     p.err_word = di.err_word; p.wait_cycles = wait_limit();
     cudaError_t err = lb::launch_gemm(pl.tile, split ? (int)lb::kEpiPartial : epi, form, maps, p, di.sms, st);
     if (err == cudaSuccess && split)
@@ -1082,9 +1082,9 @@ int lb_ffn_fwd(const void *x, const void *w_gate, const void *w_up, const void *
     }
     void *part = static_cast<char *>(workspace) + q.part;
     const Operand xs[1] = {{x, n_tok, d, d}}, w2[2] = {{w_gate, f, d, d}, {w_up, f, d, d}}, hs[2] = {{h, n_tok, f, f}, {}};
-    if ((rc = run_gemm(who, lb::kEpiGate, lb::kFormKK, q.up, xs, w2, hs, kept, nullptr, n_tok, f, d, 1, act, false, di, st))) return rc;
+    if ((rc = run_gemm(who, lb::kEpiGate, lb::kFormKK, q.up, xs, w2, hs, kept, nullptr, n_tok, f, d, 1, act, di, st))) return rc;
     const Operand wd[1] = {{w_down, d, f, f}}, ys[2] = {{y, n_tok, d, d}, {}};
-    return run_gemm(who, lb::kEpiStore, lb::kFormKK, q.down, hs, wd, ys, nullptr, part, n_tok, d, f, 1, act, true, di, st);
+    return run_gemm(who, lb::kEpiStore, lb::kFormKK, q.down, hs, wd, ys, nullptr, part, n_tok, d, f, 1, act, di, st);
 }
 
 int lb_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *h, const void *kept,
@@ -1116,20 +1116,20 @@ int lb_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *
         // dh = dy Wd, turned into dg and du as it leaves the accumulators
         const Operand wds[1] = {{w_down, d, f, f}}, outs[2] = {{dg, t, f, f2}, {du, t, f, f2}};
         if ((rc = run_gemm(who, lb::kEpiGateBwd, lb::kFormKN, q.dh, dys, wds, outs, const_cast<void *>(kept), nullptr, t, f, d, 1, 0,
-                           false, di, st))) return rc;
+                           di, st))) return rc;
     }
     if (dx) {
         const Operand as[2] = {{dg, t, f, f2}, {du, t, f, f2}}, bs[2] = {{w_gate, f, d, d}, {w_up, f, d, d}};
         const Operand cs[2] = {{dx, t, d, d}, {}};
-        if ((rc = run_gemm(who, lb::kEpiStore, lb::kFormKN, q.dx, as, bs, cs, nullptr, part, t, d, f, 2, 0, true, di, st))) return rc;
+        if ((rc = run_gemm(who, lb::kEpiStore, lb::kFormKN, q.dx, as, bs, cs, nullptr, part, t, d, f, 2, 0, di, st))) return rc;
     }
     const Operand as[2] = {{dg, t, f2, f2}, dys[0]}, bs[2] = {{x, t, d, d}, hs[0]};
     const Operand cs[2] = {{dw_gate_up, f2, d, d}, {dw_down, d, f, f}}, none[2] = {cs[1], {}};
     if (dw_gate_up && dw_down && q.together)
-        return run_gemm(who, lb::kEpiStore, lb::kFormMN, q.dw_both, as, bs, cs, nullptr, part, f2, d, t, 1, 0, true, di, st);
-    if (dw_gate_up && (rc = run_gemm(who, lb::kEpiStore, lb::kFormMN, q.dw_gu, as, bs, cs, nullptr, part, f2, d, t, 1, 0, true, di, st)))
+        return run_gemm(who, lb::kEpiStore, lb::kFormMN, q.dw_both, as, bs, cs, nullptr, part, f2, d, t, 1, 0, di, st);
+    if (dw_gate_up && (rc = run_gemm(who, lb::kEpiStore, lb::kFormMN, q.dw_gu, as, bs, cs, nullptr, part, f2, d, t, 1, 0, di, st)))
         return rc;
-    if (dw_down && (rc = run_gemm(who, lb::kEpiStore, lb::kFormMN, q.dw_down, as + 1, bs + 1, none, nullptr, part, d, f, t, 1, 0, dx || dw_gate_up, di, st)))
+    if (dw_down && (rc = run_gemm(who, lb::kEpiStore, lb::kFormMN, q.dw_down, as + 1, bs + 1, none, nullptr, part, d, f, t, 1, 0, di, st)))
         return rc;
     return LB_OK;
 }

@@ -202,6 +202,8 @@ __global__ void __launch_bounds__(kBlkThreads) block_fwd_kernel(const BlockParam
     };
     const long long step = (long long)gridDim.x * groups;
     long long tok = (long long)blockIdx.x * groups + grp;
+    grid_wait();
+    grid_launch_dependents();
     fetch(0, tok);
     fetch(1, tok + step);
     if constexpr (RES) {
@@ -350,6 +352,8 @@ __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && si
     };
     const long long step = (long long)gridDim.x * groups;
     long long tok = (long long)blockIdx.x * groups + grp;
+    grid_wait();
+    grid_launch_dependents();
     fetch(0, tok);
     fetch(1, tok + step);
     if constexpr (RES) {
@@ -493,7 +497,6 @@ __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && si
         }
     }
     if (!p.part) return;
-    grid_launch_dependents();                            // block_param_kernel's CTAs may come up as these leave
     float *mine = p.part + (long long)blockIdx.x * 2 * p.d;
     float *cols = reinterpret_cast<float *>(dyn);        // [2][d]
     cp_async_wait<0>();
@@ -530,6 +533,7 @@ template <typename W>
 __global__ void __launch_bounds__(1024) block_param_kernel(const BlockParams p, int rows) {
     __shared__ double sa[32][33], sb[32][33];
     grid_wait();
+    grid_launch_dependents();
     const int c = threadIdx.x & 31, r0 = threadIdx.x >> 5;
     const int col = blockIdx.x * 32 + c;
     double a = 0., b = 0.;
@@ -591,6 +595,8 @@ template <typename T>
 __global__ void __launch_bounds__(256, 4) dropout_kernel(const T *__restrict__ x, T *__restrict__ out, long long n, DropParams dp) {
     using S = Store<T>;
     constexpr int VEC = S::kVec;
+    grid_wait();
+    grid_launch_dependents();
     unsigned long long seed, offset;
     drop_state(dp, seed, offset);
     const KeysAdded added{(uint32_t)seed, (uint32_t)(seed >> 32)};
@@ -699,17 +705,17 @@ static cudaError_t launch_block_t(BlockParams p, bool bwd, int sms, cudaStream_t
         long long cap = (long long)sms * resident(regs[which], smem);                                                \
         if (bwd && cap > block_bwd_rows(sms)) cap = block_bwd_rows(sms);                                             \
         grid = (int)(need < cap ? need : cap);                                                                       \
-        kernel<<<grid, kBlkThreads, smem, stream>>>(p);                                                              \
+        err = launch_overlapped(kernel, dim3(grid), dim3(kBlkThreads), smem, stream, 1, p);                         \
         break;                                                                                                       \
     }
     int grid = 0;
+    cudaError_t err = cudaSuccess;
     switch (fr) {
         LB_BLK(1) LB_BLK(2) LB_BLK(3) LB_BLK(4)
     }
 #undef LB_BLK
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess || !bwd || !p.part) return e;
-    return launch_after(block_param_kernel<W>, dim3((p.d + 31) / 32), dim3(1024), 0, stream, 1, true, p, grid);
+    if (err != cudaSuccess || !bwd || !p.part) return err;
+    return launch_overlapped(block_param_kernel<W>, dim3((p.d + 31) / 32), dim3(1024), 0, stream, 1, p, grid);
 }
 
 int block_bwd_rows(int sms) { return 2 * sms < 304 ? 2 * sms : 304; }
@@ -731,11 +737,10 @@ cudaError_t launch_dropout(int dtype, const void *x, void *out, long long n, con
     const long long need = (n / vec + 1 + 255) / 256, cap = 16LL * sms;
     const int grid = (int)(need < cap ? need : cap);
     if (dtype == LB_DTYPE_BF16)
-        dropout_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16 *>(x),
-                                                                static_cast<__nv_bfloat16 *>(out), n, dp);
-    else
-        dropout_kernel<float><<<grid, 256, 0, stream>>>(static_cast<const float *>(x), static_cast<float *>(out), n, dp);
-    return cudaGetLastError();
+        return launch_overlapped(dropout_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, stream, 1, static_cast<const __nv_bfloat16 *>(x),
+                            static_cast<__nv_bfloat16 *>(out), n, dp);
+    return launch_overlapped(dropout_kernel<float>, dim3(grid), dim3(256), 0, stream, 1, static_cast<const float *>(x),
+                        static_cast<float *>(out), n, dp);
 }
 
 }  // namespace lb

@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(256) gemm_sum_kernel(const float *__restrict__
 
 cudaError_t launch_gemm_sum(const float *part, void *out, int splits, long long n, int sms, cudaStream_t stream) {
     const long long need = (n / 8 + 255) / 256, cap = 16LL * sms;
-    return launch_after(gemm_sum_kernel, dim3((unsigned)(need < cap ? need : cap)), dim3(256), 0, stream, 1, true, part,
+    return launch_overlapped(gemm_sum_kernel, dim3((unsigned)(need < cap ? need : cap)), dim3(256), 0, stream, 1, part,
                         static_cast<__nv_bfloat16 *>(out), splits, n);
 }
 

@@ -558,8 +558,8 @@ cudaError_t launch_gemm_t(const GemmMaps &maps, const GemmParams &p, int sms, cu
     const long long tiles = (long long)p.m_tiles * p.n_tiles * p.splits + (long long)p.m_tiles2 * p.n_tiles2;
     const long long groups = sms / CG;
     if (tiles < 1 || tiles + groups > 0x7fffffffLL) return cudaErrorInvalidValue;
-    return launch_after(kernel, dim3((unsigned)(CG * (tiles < groups ? tiles : groups))), dim3(Sh::kThreads), Sh::kSmem, stream, CG,
-                        p.after != 0, maps, p);
+    return launch_overlapped(kernel, dim3((unsigned)(CG * (tiles < groups ? tiles : groups))), dim3(Sh::kThreads), Sh::kSmem, stream, CG,
+                             maps, p);
 }
 
 }  // namespace lb

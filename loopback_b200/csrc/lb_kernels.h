@@ -240,7 +240,6 @@ struct GemmParams {
     int m_tiles, n_tiles, splits;
     int m2, n2, m_tiles2, n_tiles2;   // kFormMN: a second product over the same k in the same launch (m_tiles2 = 0: none)
     int act;                  // LB_ACT_*
-    int after;                // launched behind another kernel of the same call (see lb_launch.cuh)
     int test_skip_item;       // test hook: the first CTA's k-th copy of A is left out (0 = off)
     uint8_t *kept;            // act'(g) u and act(g) in blocks of 32 x 32 (kEpiGate: null = not kept)
     int *err_word;
@@ -262,7 +261,7 @@ constexpr int kGemmTileCount = 3;
 
 cudaError_t launch_gemm(int tile, int epilogue, int form, const GemmMaps &maps, const GemmParams &p, int sms, cudaStream_t stream);
 // the same block for few rows (lb_ffn_small.cu)
-constexpr int kFfnSmallTokens = 128;               // rows at most
+constexpr int kFfnSmallTokens = 64;                // rows at most
 struct FfnSmallParams {
     void *out;                // [n_tok][n]: h or y
     int n_tok, n;             // n: columns of the result (= weight rows of one projection)

@@ -1,6 +1,8 @@
-// Launches that follow one another on a stream: a kernel launched `after` its predecessor may have its CTAs set up while the
-// predecessor's last ones run (programmatic stream serialisation). Such a kernel calls grid_wait() before it touches anything
-// another kernel wrote or reads: that waits for the predecessor's end, its memory included.
+// Launches whose edges overlap: with programmatic stream serialisation a kernel's CTAs may come up while the last ones of the
+// kernel before it on the stream still run, where that one allows it (grid_launch_dependents; the end of a kernel that does
+// not). Such a kernel calls grid_wait() before it touches memory that another kernel wrote or reads: that waits for the
+// predecessor's end, its memory included. A kernel allows its successors only behind its own grid_wait(), so that a kernel's
+// end means the end of everything before it.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -11,7 +13,7 @@ __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <typename Kernel, typename... Args>
-cudaError_t launch_after(Kernel kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, int cluster, bool after, Args... args) {
+cudaError_t launch_overlapped(Kernel kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, int cluster, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -25,11 +27,9 @@ cudaError_t launch_after(Kernel kernel, dim3 grid, dim3 block, size_t smem, cuda
         at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
         ++n;
     }
-    if (after) {
-        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[n].val.programmaticStreamSerializationAllowed = 1;
-        ++n;
-    }
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
     cfg.attrs = at;
     cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kernel, args...);

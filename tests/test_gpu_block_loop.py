@@ -162,3 +162,81 @@ def test_a_pass_in_a_graph_draws_new_masks():
         assert all(torch.equal(a, b) for a, b in zip(mine, want))
         seen.append(mine[0])
     assert not torch.equal(*seen)
+
+
+def _chain(x, block, rng):
+    """Every kind of launch of the operators behind one another, each result from the one before."""
+    from loopback_b200 import block as B
+    u = B.block_norm(x, block.norm)
+    y = B.dropout(B.gated_ffn(u, block.w_gate, block.w_up, block.w_down), 0.25, rng)
+    out, n = B.block_residual(x, y, block.norm_after, gate=block.gate, scale=0.5, next_weight=block.norm, p=0.1, rng=rng)
+    return out, n
+
+
+@pytest.mark.parametrize("t", [1, 64, 300, 5000])
+@pytest.mark.parametrize("before", ["nothing", "copy", "fill", "memset", "host copy", "other stream", "own kernel"])
+def test_launches_wait_for_what_comes_before(t, before):
+    """The launches overlap their edges with whatever precedes them on the stream, eager and captured: what an earlier piece of
+    work still writes when the operator is launched (weights and rows, behind a long kernel) has to be what it reads."""
+    blocks, _ = _model(6)
+    block = blocks[2]
+    gen = torch.Generator(device="cuda").manual_seed(t)
+    x = torch.randn(t, D, device="cuda", generator=gen).bfloat16()
+    rng = torch.tensor([5, 6], device="cuda")
+    side = torch.cuda.Stream()
+    host = x.cpu().pin_memory()
+    with torch.no_grad():
+        want = _chain(x, block, rng)
+        good = {n: v.clone() for n, v in block.named_parameters()}
+        wrong, late = torch.zeros_like(x), torch.full_like(x, 9.0)
+        names = ("w_gate", "w_up", "w_down", "norm")
+
+        def spoil():
+            late.fill_(9.0)
+            for n in names:
+                getattr(block, n).fill_(3.0)
+
+        def put(v):                                       # a slow kernel, then what the chain reads
+            torch.cuda._sleep(200_000)
+            for n in names:
+                getattr(block, n).copy_(good[n])
+            if v == "copy":
+                late.copy_(x)
+            elif v == "fill":
+                late.copy_(x)
+                wrong.fill_(1.0)
+            elif v == "memset":
+                late.copy_(x)
+                wrong.zero_()
+            elif v == "host copy":
+                late.copy_(host, non_blocking=True)
+            elif v == "other stream":
+                side.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(side):
+                    torch.cuda._sleep(100_000)
+                    late.copy_(x)
+                torch.cuda.current_stream().wait_stream(side)
+            elif v == "own kernel":
+                from loopback_b200 import block as B
+                late.copy_(x)
+                B.block_norm(late, block.norm)
+        if before != "nothing":
+            for _ in range(3):
+                spoil()
+                put(before)
+                got = _chain(late, block, rng)
+                torch.cuda.synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(got, want))
+        graph = torch.cuda.CUDAGraph()
+        late.copy_(x)
+        with torch.cuda.graph(graph):
+            if before != "nothing":
+                put(before)
+            got = _chain(late, block, rng)
+            again = _chain(late, block, rng)              # its own launches precede it
+        for _ in range(3):
+            if before != "nothing":
+                spoil()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.equal(a, b) for a, b in zip(again, want))
