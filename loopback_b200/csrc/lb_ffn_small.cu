@@ -15,6 +15,9 @@
 //                31 instead of 23 at 64 rows.)
 #include "lb_gemm.cuh"
 
+// 1 x 2048 x 5632: 69 MB in 18.1 us where the copy rate would take 10.6; the rest is the two launches' edges and the wait for h
+// between them (4096 x 11008: 47.6 of 41.3).
+
 namespace lb {
 
 constexpr int kSmallThreads = 192;
