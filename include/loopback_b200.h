@@ -62,8 +62,9 @@ int lb_device_error(int clear);
  * tiled write kernel, whatever the batch size; 3: the tensor-core write kernel whatever the batch size),
  * "write_mt" (16-token tiles per consumer warp of the tensor-core write kernel: 1 or 2),
  * "write_tile" (tokens per tile of the tensor-core write kernel: a multiple of 32 up to 256), "write_stages" (its TMA
- * ring depth, 2..8), "fwd_sps" (sources per TMA stage of the forward read: 1, 2 or 4), "ffn_tile" (tile shape of the feed-forward products, 1..: an
- * index into the shapes they are built for), "ffn_splits" (slices along k, where a product may be split), "ffn_small" (rows up to which a forward without
+ * ring depth, 2..8), "fwd_sps" (sources per TMA stage of the forward read: 1, 2 or 4), "ffn_tile" (tile shape of the feed-forward products: 1
+ * 128 x 128, 2 128 x 256, 3 256 x 256, 4 128 x 128 with k split over a cluster, where a product may be split), "ffn_splits"
+ * (parts of k, where a product may be split), "ffn_small" (rows up to which a forward without
  * gradients takes the kernels for few rows; -1 never), "block_frags" (16-byte fragments of a row per lane of the
  * norm and residual kernels at most: 1..4), "wait_cycles" (the limit of
  * every bounded wait inside the kernels, in GPU clock cycles; default 4e9), "test_skip_item" (test hook: the first
@@ -309,7 +310,7 @@ int lb_dropout(const void *x, void *out, int threshold, const int64_t *rng, int6
 /* The gated feed-forward block: g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T. x, y [n_tok][d]; Wg, Wu [f][d] and
  * Wd [d][f] (torch's Linear layout); everything bf16, products on the tensor cores with fp32 accumulation, h and y rounded
  * once each. d and f are multiples of 8. The block is two launches (both projections, the activation and the product in
- * the first), or three where the second is split along f. */
+ * the first), or three where the second is split along f in slices through the workspace (a few tiles split it inside a cluster). */
 #define LB_ACT_SILU 0 /* g / (1 + exp(-g)) */
 #define LB_ACT_GELU 1 /* g (1 + erf(g / sqrt 2)) / 2 */
 

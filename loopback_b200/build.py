@@ -21,7 +21,7 @@ TORCH_SRC = os.path.join(CSRC, "lb_torch.cpp")
 TORCH_LIB = os.path.join(HERE, "_torch_ops.so")
 SOURCES = ("lb_api.cu", "lb_write.cu", "lb_write_mma.cu", "lb_read_fwd.cu", "lb_read_bwd.cu", "lb_read_bwd_f32.cu", "lb_step.cu",
            "lb_noalloc.cu", "lb_peer.cu", "lb_block.cu", "lb_ffn.cu", "lb_ffn_small.cu",
-           "lb_gemm_kk.cu", "lb_gemm_kn.cu", "lb_gemm_mn.cu")
+           "lb_gemm_cluster.cu", "lb_gemm_kk.cu", "lb_gemm_kn.cu", "lb_gemm_mn.cu")
 HEADERS = ("lb_common.cuh", "lb_kernels.h", "lb_read_bwd_impl.cuh", "lb_gemm.cuh", "lb_launch.cuh", os.path.join("..", "..", "include", "loopback_b200.h"))
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden", "-ccbin", "g++",

@@ -902,6 +902,7 @@ static int make_map_part(CUtensorMap *m, void *base, long long rows, long long c
 
 struct GemmPlan {
     int tile = 0, splits = 1;
+    bool cluster = false;              // k split over the CTAs of a cluster, no slices
     int m_tiles = 0, n_tiles = 0, m_tiles2 = 0, n_tiles2 = 0;
     double us = 1e30;                  // estimated
 };
@@ -924,14 +925,31 @@ static GemmPlan plan_gemm(long long m, long long n, long long blocks, bool gate,
             // 256-row one by the tensor cores), a launch's fixed part, and the slices' way out and in
             const double rate = cg == 2 ? 0.345 : bn == 256 ? 0.39 : 0.30;
             double us = waves * (double)((blocks + s - 1) / s) * rate + 4.5 + bn / 128. + (cg == 2 ? 1.0 : 0.0);
-            if (s > 1) us += 2.0 + (double)s * m * n * 8. / 5.0e6;
+            if (s > 1) us += 2.0 + (double)s * m * n * 8. / 9.0e6;
             if (us < best.us) {
-                best.us = us; best.tile = i; best.splits = s;
+                best.us = us; best.tile = i; best.splits = s; best.cluster = false;
                 best.m_tiles = (int)mt; best.n_tiles = (int)nt; best.m_tiles2 = (int)mt2; best.n_tiles2 = (int)nt2;
             }
         }
     }
     return best;
+}
+
+// ... and the same with k split over a cluster, where the whole product is resident at once (two CTAs to an SM, less what the
+// clusters' shapes leave unused). The constants are fitted to 100 .. 2048 rows of 768 .. 2048 columns over 32 .. 88 blocks.
+static void plan_cluster(GemmPlan *best, long long m, long long n, long long blocks, int sms) {
+    if (g_opt.ffn_tile > 0 && g_opt.ffn_tile != lb::kGemmTileCount + 1) return;
+    const long long mt = (m + 127) / 128, nt = (n + 127) / 128;
+    const int most = blocks / 2 < lb::kClusterSplits ? (int)(blocks / 2) : lb::kClusterSplits;
+    for (int s = 2; s <= most && mt * nt * s * 4 <= 7LL * sms; ++s) {
+        if (g_opt.ffn_splits > 0 && s != (g_opt.ffn_splits < most ? g_opt.ffn_splits : most)) continue;
+        const double full = (double)(mt * nt * s) / sms;
+        const double us = 5.5 + (full > 1.0 ? 0.50 : 0.25 + 0.10 * full) * (double)((blocks + s - 1) / s) + 0.45 * s;
+        if (us < best->us || g_opt.ffn_tile == lb::kGemmTileCount + 1) {
+            best->us = us; best->tile = 0; best->splits = s; best->cluster = true;
+            best->m_tiles = (int)mt; best->n_tiles = (int)nt; best->m_tiles2 = best->n_tiles2 = 0;
+        }
+    }
 }
 
 struct Operand {
@@ -949,7 +967,7 @@ static int run_gemm(const char *who, int epi, int form, const GemmPlan &pl, cons
     lb::GemmParams p;
     const int cg = lb::kGemmTiles[pl.tile].cg, bn = lb::kGemmTiles[pl.tile].bn;
     int rc;
-    const bool split = pl.splits > 1, two = pl.m_tiles2 > 0;
+    const bool split = pl.splits > 1 && !pl.cluster, two = pl.m_tiles2 > 0;
     const int pairs = two ? 2 : segs;
     for (int s = 0; s < pairs; ++s)
         if ((rc = make_map_tile(&maps.a[s], a[s].base, a[s].rows, a[s].cols, a[s].ld, form == lb::kFormMN ? 64 : 128))) return rc;
@@ -967,6 +985,10 @@ static int run_gemm(const char *who, int epi, int form, const GemmPlan &pl, cons
     p.m_tiles = pl.m_tiles; p.n_tiles = pl.n_tiles; p.splits = pl.splits; p.m_tiles2 = pl.m_tiles2; p.n_tiles2 = pl.n_tiles2;
     p.m2 = two ? (int)c[1].rows : 0; p.n2 = two ? (int)c[1].cols : 0; p.act = act; p.test_skip_item = g_opt.test_skip_item; p.kept = static_cast<uint8_t *>(kept);
     p.err_word = di.err_word; p.wait_cycles = wait_limit();
+    if (pl.cluster) {
+        const cudaError_t e = lb::launch_gemm_cluster(form, maps, p, const_cast<void *>(c[0].base), st);
+        return e == cudaSuccess ? LB_OK : cuda_fail(e, who);
+    }
     cudaError_t err = lb::launch_gemm(pl.tile, split ? (int)lb::kEpiPartial : epi, form, maps, p, di.sms, st);
     if (err == cudaSuccess && split)
         err = lb::launch_gemm_sum(static_cast<const float *>(part), const_cast<void *>(c[0].base), pl.splits, m * n, di.sms, st);
@@ -995,18 +1017,22 @@ static FfnPlan plan_ffn(long long t, long long d, long long f, int kind, int sms
     const auto blocks = [](long long k) { return (k + 63) / 64; };
     size_t part = 0;
     const auto need = [&](const GemmPlan &g, long long m, long long n) {
-        const size_t b = g.splits > 1 ? (size_t)g.splits * (size_t)m * (size_t)n * 4 : 0;
+        const size_t b = g.splits > 1 && !g.cluster ? (size_t)g.splits * (size_t)m * (size_t)n * 4 : 0;
         if (b > part) part = b;
     };
     if (!bwd) {
         q.up = plan_gemm(t, f, blocks(d), true, false, sms);
         q.down = plan_gemm(t, d, blocks(f), false, true, sms);
+        plan_cluster(&q.down, t, d, blocks(f), sms);
         need(q.down, t, d);
     } else {
         q.dh = plan_gemm(t, f, blocks(d), false, false, sms);
         q.dx = plan_gemm(t, d, 2 * blocks(f), false, true, sms);
         q.dw_gu = plan_gemm(2 * f, d, blocks(t), false, true, sms);
         q.dw_down = plan_gemm(d, f, blocks(t), false, true, sms);
+        plan_cluster(&q.dx, t, d, 2 * blocks(f), sms);
+        plan_cluster(&q.dw_gu, 2 * f, d, blocks(t), sms);
+        plan_cluster(&q.dw_down, d, f, blocks(t), sms);
         // the two weight gradients are sums over the same rows: in one launch their tiles fill the last round together
         // (8192 x 1024 x 2816: 134 us apart)
         q.dw_both = plan_gemm(2 * f, d, blocks(t), false, false, sms, d, f);

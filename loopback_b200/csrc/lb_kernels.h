@@ -260,6 +260,9 @@ constexpr GemmTile kGemmTiles[] = {{1, 128}, {1, 256}, {2, 256}};
 constexpr int kGemmTileCount = 3;
 
 cudaError_t launch_gemm(int tile, int epilogue, int form, const GemmMaps &maps, const GemmParams &p, int sms, cudaStream_t stream);
+// the product of tile shape 0 split along k over clusters of p.splits CTAs (2..8), one tile each (lb_gemm_cluster.cu)
+constexpr int kClusterSplits = 8;
+cudaError_t launch_gemm_cluster(int form, const GemmMaps &maps, const GemmParams &p, void *out, cudaStream_t stream);
 // the same block for few rows (lb_ffn_small.cu)
 constexpr int kFfnSmallTokens = 64;                // rows at most
 struct FfnSmallParams {

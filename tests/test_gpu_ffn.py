@@ -36,7 +36,7 @@ SIZES = [(128, 64, 128), (128, 128, 256), (256, 256, 512), (1, 8, 8), (1, 64, 64
          (129, 768, 2048), (255, 1000, 136), (257, 264, 520), (300, 8, 1032), (300, 1032, 8), (1000, 512, 1408)]
 
 
-@pytest.mark.parametrize("tile", [1, 2, 3])
+@pytest.mark.parametrize("tile", [1, 2, 3, 4])
 @pytest.mark.parametrize("t,d,f", SIZES)
 def test_training_sizes(t, d, f, tile):
     import loopback_b200._lib as L
@@ -47,14 +47,14 @@ def test_training_sizes(t, d, f, tile):
         L.reset_options()
 
 
-@pytest.mark.parametrize("tile", [1, 2, 3])
-@pytest.mark.parametrize("splits", [1, 2, 5])
-def test_splits_along_k(tile, splits):
+@pytest.mark.parametrize("tile,t", [(1, 1400), (2, 1400), (3, 1400), (4, 700)])
+@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8])
+def test_splits_along_k(tile, t, splits):
     import loopback_b200._lib as L
     try:
         L.set_option("ffn_tile", tile)
         L.set_option("ffn_splits", splits)
-        _check(1400, 264, 1288, seed=splits)
+        _check(t, 264, 1288, seed=splits)
     finally:
         L.reset_options()
 
@@ -213,7 +213,7 @@ def test_on_another_stream_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(grads, want))
 
 
-@pytest.mark.parametrize("t,tile", [(300, 1), (300, 3), (40, 0)])
+@pytest.mark.parametrize("t,tile", [(300, 1), (300, 3), (300, 4), (40, 0)])
 def test_a_wait_that_runs_out_unwinds_and_reports(t, tile):
     """The products' waits are bounded. With the limit at about a millisecond and the hook that leaves out one tile copy of the
     first CTA, its multiplies give up, everybody unwinds, the kernel returns and the device error word names a wait; the next
