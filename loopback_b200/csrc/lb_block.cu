@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && si
             float3 sums = row_sums(make_float3(s1.x + s1.y, s2.x + s2.y, s3.x + s3.y), wpt, grp, wl, lane, slots3, turn);
             const float mean = sums.x * inv_d, S1 = fmaf(-ro * mean, sums.z, sums.y);
             if (p.gate_kind == kGateToken && p.dgate && wl == 0 && lane == 0) S::store1(static_cast<T *>(p.dgate) + tok, s * S1);
-            const float2 c1 = splat(-mean), k1 = splat(s * gt * ry), c2 = splat(w ? -S1 * inv_d : 0.f);
+            const float2 c1 = splat(-mean), k1 = splat(s * gt * ry), c2 = splat(-S1 * inv_d);
 #pragma unroll
             for (int k = 0; k < FR; ++k) {
                 if (f0 + 32 * k >= p.frags) continue;
@@ -476,6 +476,7 @@ __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && si
                 if (dx) st_global_v4(dx + row + k * 32 * VEC, S::pack2v(D[k]));
                 if (drop) drop_pairs<P>(D[k], words[k], p.drop.threshold);
                 S::unpack2(lds_v4(slot(stage, 2, k)), yh);
+                if (drop && !w) drop_pairs<P>(yh, words[k], p.drop.threshold);      // what is dropped may be anything
 #pragma unroll
                 for (int i = 0; i < P; ++i) yh[i] = __fmul2_rn(yh[i], ry2);
                 channel_pairs<P>(v, tab_wg + k * 512, plane);
@@ -489,13 +490,20 @@ __global__ void __launch_bounds__(kBlkThreads, FR <= 2 || !RES || (FR == 3 && si
                     S::unpack2(lds_v4(slot(stage, 4, k)), g);
 #pragma unroll
                     for (int i = 0; i < P; ++i) D[k][i] = __fmul2_rn(D[k][i], g[i]);
+                    if (drop) drop_pairs<P>(D[k], words[k], p.drop.threshold);
                 }
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
                     const float2 a = p.gate_kind == kGateToken ? __fmul2_rn(splat(gt), D[k][i]) : D[k][i];
                     colA[k][i] = __ffma2_rn(a, yh[i], colA[k][i]);
-                    D[k][i] = __fmul2_rn(k1, __ffma2_rn(c2, yh[i], __fmul2_rn(D[k][i], v[i])));
+                    D[k][i] = __fmul2_rn(D[k][i], v[i]);
                 }
+                if (w) {                                 // without the norm dy does not depend on y, which may be infinite
+#pragma unroll
+                    for (int i = 0; i < P; ++i) D[k][i] = __ffma2_rn(c2, yh[i], D[k][i]);
+                }
+#pragma unroll
+                for (int i = 0; i < P; ++i) D[k][i] = __fmul2_rn(k1, D[k][i]);
                 if (dy) st_global_v4(dy + row + k * 32 * VEC, S::pack2v(D[k]));
             }
             fetch(stage, tok + 2 * step);

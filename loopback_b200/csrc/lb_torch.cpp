@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -102,6 +103,22 @@ void channel_params(const Tensor &x, std::initializer_list<Tensor *> ps, const c
         if (p->defined()) *p = dense(cast ? p->to(at::kFloat) : *p);
 }
 
+// The engine hands a gradient over on the stream of the node that takes it. While a backward is captured that must not be the
+// default stream, which cannot be part of a capture: a leaf's node was made there where an eager graph of the same leaf is still
+// alive. The engine's own error would end the process; this one is raised before it, and the capture ends in order.
+void check_capture(const char *what) {
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    for (size_t i = 0; i < node->num_outputs(); ++i) {
+        if (!node->task_should_compute_output(i)) continue;
+        const auto s = node->next_edge(i).function->stream();
+        TORCH_CHECK(!s || s->device_type() != c10::DeviceType::CUDA || c10::cuda::CUDAStream(*s).stream() != nullptr, "loopback_b200.", what,
+                    ": this backward is captured into a CUDA graph, but an input's gradient belongs to the default stream: an eager "
+                    "autograd graph of the same tensor is alive. Release its results before the capture, or record it on another stream");
+    }
+}
+
 // Under create_graph the results of a backward would be taken for constants: they raise where somebody differentiates them.
 variable_list once(variable_list grads, const char *what) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -132,6 +149,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
         return u;
     }
     static variable_list backward(AutogradContext *ctx, variable_list g) {
+        check_capture("block_norm");
         const variable_list s = ctx->get_saved_variables();
         const Tensor &x = s[0], &w = s[1], &r = s[2];
         const int64_t d = x.size(-1);
@@ -186,6 +204,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
         return out;
     }
     static variable_list backward(AutogradContext *ctx, variable_list g) {
+        check_capture("dropout");
         const Tensor used = ctx->get_saved_variables()[0];
         Tensor dx = dropout_launch(dense(g[0]), ctx->saved_data["threshold"].toInt(), used, ctx->saved_data["seed"].toInt(),
                                    ctx->saved_data["offset"].toInt(), Tensor());
@@ -251,6 +270,7 @@ struct BlockResidual : torch::autograd::Function<BlockResidual> {
         return got;
     }
     static variable_list backward(AutogradContext *ctx, variable_list g) {
+        check_capture("block_residual");
         const variable_list s = ctx->get_saved_variables();
         const Tensor &x = s[0], &y = s[1], &w = s[2], &gate = s[3], &scale = s[4], &next_w = s[5], &stats = s[6];
         const Tensor g_out = g[0].defined() ? dense(g[0]) : Tensor();
@@ -347,6 +367,7 @@ struct GatedFFN : torch::autograd::Function<GatedFFN> {
         return y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list g) {
+        check_capture("gated_ffn");
         const variable_list s = ctx->get_saved_variables();
         const Tensor &x = s[0], &wg = s[1], &wu = s[2], &wd = s[3], &h = s[4], &kept = s[5];
         const int64_t d = x.size(-1), f = wg.size(0), n = x.numel() / d;

@@ -195,6 +195,36 @@ def test_dropout_clears_what_it_drops():
     assert torch.equal(out == 1, (m == 0).view(4, 1024))
 
 
+@pytest.mark.parametrize("after", [False, True])
+@pytest.mark.parametrize("kind", ["", "channel", "token", "full"])
+@pytest.mark.parametrize("types", list(TYPES))
+def test_dropped_values_reach_no_gradient(types, kind, after):
+    """Without a norm after the block, what y (and a gate per element) holds where it is dropped changes no bit of any result."""
+    t, d, p = 37, 264, 0.4
+    finite = _residual_case(types, t, d, False, kind, True, after, p, 6)
+    dropped = (ref.factor(p, int(finite["rng"][0]), int(finite["rng"][1]), 0, t * d) == 0).view(t, d).cuda()
+    clone = lambda v: v.detach().clone() if isinstance(v, torch.Tensor) else v  # noqa: E731
+    for bad in (float("inf"), float("nan")):
+        s = {k: clone(v) for k, v in finite.items()}
+        s["y"][dropped] = bad
+        if kind == "full":
+            s["gate"][dropped] = bad
+        want, got = _run_residual({k: clone(v) for k, v in finite.items()}, p), _run_residual(s, p)
+        for k, v in got.items():
+            assert torch.isfinite(v).all(), k
+            assert torch.equal(v, want[k]), k
+
+
+@pytest.mark.parametrize("types", list(TYPES))
+def test_infinite_branch_without_a_norm_has_a_finite_gradient(types):
+    """out = x + s y: dy = s dout whatever y holds."""
+    s = _residual_case(types, 9, 136, False, "", False, False, 0.0, 2)
+    want = _run_residual(dict(s), 0.0)["dy"]
+    y = s["y"].detach().clone()
+    y[3, 5], y[8, 135] = float("inf"), float("nan")
+    assert torch.equal(_run_residual({**s, "y": y}, 0.0)["dy"], want)
+
+
 def test_dropout_past_32_bits_of_elements():
     from loopback_b200 import block
     n = (1 << 32) + 1024 + 5

@@ -240,3 +240,45 @@ def test_launches_wait_for_what_comes_before(t, before):
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.equal(a, b) for a, b in zip(again, want))
+
+
+_CAPTURE = """
+import torch
+from loopback_b200 import block as B
+x = torch.randn(300, 64, device="cuda").bfloat16().requires_grad_()
+w, wg, wu, wd = (torch.randn(*s, device="cuda").bfloat16().requires_grad_() for s in ((64,), (128, 64), (128, 64), (64, 128)))
+calls = {"block_norm": (lambda: B.block_norm(x, w), (x, w)), "dropout": (lambda: B.dropout(x, 0.5, (1, 2)), (x,)),
+         "block_residual": (lambda: B.block_residual(x, x, w, p=0.5, rng=(1, 2)), (x, w)),
+         "gated_ffn": (lambda: B.gated_ffn(x, wg, wu, wd), (x, wg, wu, wd))}
+up = torch.ones_like(x)
+for name, (call, leaves) in calls.items():
+    alive = call()                                       # its graph holds the leaves' nodes, on the default stream
+    want = torch.autograd.grad(alive, leaves, up, retain_graph=True)
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(call(), leaves, up)
+        raise SystemExit(name + " was captured")
+    except RuntimeError as e:
+        assert "is alive" in str(e), e
+    again = torch.autograd.grad(alive, leaves, up)       # the eager graph is as it was
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(call(), leaves, up)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, again, got)), name
+print("refused and captured")
+"""
+
+
+def test_capture_of_a_backward_beside_a_live_eager_graph():
+    """The backward of leaves whose eager graph is alive cannot be captured: it raises, and works once that graph is gone. In a
+    child process, since the error it stands in front of would end this one."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", _CAPTURE], capture_output=True, text=True, timeout=300, cwd=here)
+    assert done.returncode == 0 and "refused and captured" in done.stdout, done.stdout[-2000:] + done.stderr[-2000:]

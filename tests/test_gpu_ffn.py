@@ -48,7 +48,7 @@ def test_training_sizes(t, d, f, tile):
 
 
 @pytest.mark.parametrize("tile,t", [(1, 1400), (2, 1400), (3, 1400), (4, 700)])
-@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("splits", [1, 2, 3, 5, 6, 7, 8])
 def test_splits_along_k(tile, t, splits):
     import loopback_b200._lib as L
     try:
