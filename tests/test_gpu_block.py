@@ -236,6 +236,27 @@ def test_dropout_past_32_bits_of_elements():
         assert torch.equal(out[at:at + len(m)].double(), m)
 
 
+def test_rows_past_32_bits_of_elements():
+    """Rows are independent: those behind 2^32 elements have the bits of a small batch of the same rows."""
+    from loopback_b200 import block
+    d, few = 1024, 4096
+    t = (1 << 32) // d + 5
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    xs, ys = (_rows(gen, few, d, torch.bfloat16) for _ in range(2))
+    w, wn = (_weight(gen, d, torch.bfloat16) for _ in range(2))
+    up = torch.ones(t, d, device="cuda", dtype=torch.bfloat16)
+
+    def run(x, y):
+        x.requires_grad_(), y.requires_grad_()
+        out, u = block.block_residual(x, y, w, scale=0.5, next_weight=wn)
+        return [out.detach(), u.detach(), *torch.autograd.grad((out, u), (x, y), (up[:len(x)],) * 2)]
+
+    want = run(xs, ys)
+    got = run(*(torch.cat((v.detach().repeat(t // few, 1), v.detach()[:t % few])) for v in (xs, ys)))
+    for a, b in zip(want, got):
+        assert torch.equal(b[:few], a) and torch.equal(b[-(t % few) - few:-(t % few)], a) and torch.equal(b[-(t % few):], a[:t % few])
+
+
 def test_dropout_same_mask_in_the_residual():
     """block_residual's dropout is dropout() of the branch: without a norm and with x = 0 the two give the same bits."""
     from loopback_b200 import block

@@ -161,6 +161,20 @@ def test_large_activations():
             assert bool((off <= want[k][1] + 2.0 ** -8 * (want[k][0].abs() + want[k][1]) + 1e-30).all()), (act, k)
 
 
+def test_hidden_past_32_bits_of_elements():
+    """What is kept between the products passes 2^32 elements: the last rows' result and gradient are right."""
+    from loopback_b200 import block
+    d, f, few = 64, 4096, 300
+    t = (1 << 32) // f + few
+    (x, wg, wu, wd), dy = _inputs(t, d, f, 3)
+    y = block.gated_ffn(x, wg.detach(), wu.detach(), wd.detach())
+    (dx,) = torch.autograd.grad(y, x, dy)
+    for rows in (slice(0, few), slice(t // 2 - few, t // 2), slice(t - few, t)):
+        want = ref.ffn(*(v.detach().double() for v in (x[rows], wg, wu, wd)), "silu", dy[rows].double())
+        ref.check_ffn("y", y[rows].detach(), *want["y"])
+        ref.check_ffn("dx", dx[rows], *want["dx"])
+
+
 def test_shapes_frozen_weights_and_empty_batches():
     from loopback_b200 import block
     (x, wg, wu, wd), dy = _inputs(60, 72, 136, 1)
