@@ -63,8 +63,8 @@ int lb_device_error(int clear);
  * "write_mt" (16-token tiles per consumer warp of the tensor-core write kernel: 1 or 2),
  * "write_tile" (tokens per tile of the tensor-core write kernel: a multiple of 32 up to 256), "write_stages" (its TMA
  * ring depth, 2..8), "fwd_sps" (sources per TMA stage of the forward read: 1, 2 or 4), "ffn_tile" (tile shape of the feed-forward products: 1
- * 128 x 128, 2 128 x 256, 3 256 x 256, 4 128 x 128 with k split over a cluster, where a product may be split), "ffn_splits"
- * (parts of k, where a product may be split), "ffn_small" (rows up to which a forward without
+ * 128 x 128, 2 128 x 256, 3 256 x 256, 4 256 x 512 (not the gated ones), 5 128 x 128 with k split over a cluster, where a
+ * product may be split), "ffn_splits" (parts of k, where a product may be split), "ffn_small" (rows up to which a forward without
  * gradients takes the kernels for few rows; -1 never), "block_frags" (16-byte fragments of a row per lane of the
  * norm and residual kernels at most: 1..4), "wait_cycles" (the limit of
  * every bounded wait inside the kernels, in GPU clock cycles; default 4e9), "test_skip_item" (test hook: the first

@@ -909,21 +909,23 @@ struct GemmPlan {
 
 // Tile shape and split along k of an m x n product over `blocks` blocks of 64 (and an m2 x n2 one beside it): the least
 // estimated time.
-static GemmPlan plan_gemm(long long m, long long n, long long blocks, bool gate, bool may_split, int sms, long long m2 = 0,
+static GemmPlan plan_gemm(long long m, long long n, long long blocks, int epi, bool may_split, int sms, long long m2 = 0,
                           long long n2 = 0) {
     GemmPlan best;
-    for (int i = 0; i < lb::kGemmTileCount; ++i) {
-        if (g_opt.ffn_tile > 0 && g_opt.ffn_tile <= lb::kGemmTileCount && g_opt.ffn_tile - 1 != i) continue;
+    const bool gate = epi == lb::kEpiGate, plain = epi == lb::kEpiStore;
+    const int shapes = lb::kGemmTileCount - !plain;                    // the last one is for plain products
+    for (int i = 0; i < shapes; ++i) {
+        if (g_opt.ffn_tile > 0 && g_opt.ffn_tile <= shapes && g_opt.ffn_tile - 1 != i) continue;
         const int cg = lb::kGemmTiles[i].cg, bn = lb::kGemmTiles[i].bn;
         const long long tm = 128LL * cg, tn = gate ? bn / 2 : bn, groups = sms / cg;
         const long long mt = (m + tm - 1) / tm, nt = (n + tn - 1) / tn, mt2 = (m2 + tm - 1) / tm, nt2 = (n2 + tn - 1) / tn;
-        const int most = !may_split || blocks < 8 ? 1 : blocks / 4 < 16 ? (int)(blocks / 4) : 16;
-        const int forced = g_opt.ffn_splits <= 0 || !may_split ? 0 : g_opt.ffn_splits < most ? g_opt.ffn_splits : most;
+        const int most = !may_split || blocks < 8 || bn > 256 ? 1 : blocks / 4 < 16 ? (int)(blocks / 4) : 16;
+        const int forced = g_opt.ffn_splits <= 0 || most == 1 ? 0 : g_opt.ffn_splits < most ? g_opt.ffn_splits : most;
         for (int s = forced ? forced : 1; s <= (forced ? forced : most); ++s) {
             const double waves = (double)((mt * nt * s + mt2 * nt2 + groups - 1) / groups);
             // us per block of 64 of a tile, as measured with the SMs busy (a 128 x 128 tile is bound by what L2 delivers, the
-            // 256-row one by the tensor cores), a launch's fixed part, and the slices' way out and in
-            const double rate = cg == 2 ? 0.345 : bn == 256 ? 0.39 : 0.30;
+            // 256-row ones by the tensor cores), a launch's fixed part, and the slices' way out and in
+            const double rate = bn == 512 ? 0.58 : cg == 2 ? 0.345 : bn == 256 ? 0.39 : 0.30;
             double us = waves * (double)((blocks + s - 1) / s) * rate + 4.5 + bn / 128. + (cg == 2 ? 1.0 : 0.0);
             if (s > 1) us += 2.0 + (double)s * m * n * 8. / 9.0e6;
             if (us < best.us) {
@@ -973,7 +975,7 @@ static int run_gemm(const char *who, int epi, int form, const GemmPlan &pl, cons
         if ((rc = make_map_tile(&maps.a[s], a[s].base, a[s].rows, a[s].cols, a[s].ld, form == lb::kFormMN ? 64 : 128))) return rc;
     for (int s = 0; s < (epi == lb::kEpiGate ? 2 : pairs); ++s)
         if ((rc = make_map_tile(&maps.b[s], b[s].base, b[s].rows, b[s].cols, b[s].ld,
-                                form != lb::kFormKK ? 64 : epi == lb::kEpiGate ? bn / 2 : bn / cg))) return rc;
+                                form != lb::kFormKK ? 64 : epi == lb::kEpiGate ? bn / 2 : (bn < 256 ? bn : 256) / cg))) return rc;
     if (split) {
         if ((rc = make_map_part(&maps.c[0], part, m, n, pl.splits))) return rc;
     } else {
@@ -1021,21 +1023,21 @@ static FfnPlan plan_ffn(long long t, long long d, long long f, int kind, int sms
         if (b > part) part = b;
     };
     if (!bwd) {
-        q.up = plan_gemm(t, f, blocks(d), true, false, sms);
-        q.down = plan_gemm(t, d, blocks(f), false, true, sms);
+        q.up = plan_gemm(t, f, blocks(d), lb::kEpiGate, false, sms);
+        q.down = plan_gemm(t, d, blocks(f), lb::kEpiStore, true, sms);
         plan_cluster(&q.down, t, d, blocks(f), sms);
         need(q.down, t, d);
     } else {
-        q.dh = plan_gemm(t, f, blocks(d), false, false, sms);
-        q.dx = plan_gemm(t, d, 2 * blocks(f), false, true, sms);
-        q.dw_gu = plan_gemm(2 * f, d, blocks(t), false, true, sms);
-        q.dw_down = plan_gemm(d, f, blocks(t), false, true, sms);
+        q.dh = plan_gemm(t, f, blocks(d), lb::kEpiGateBwd, false, sms);
+        q.dx = plan_gemm(t, d, 2 * blocks(f), lb::kEpiStore, true, sms);
+        q.dw_gu = plan_gemm(2 * f, d, blocks(t), lb::kEpiStore, true, sms);
+        q.dw_down = plan_gemm(d, f, blocks(t), lb::kEpiStore, true, sms);
         plan_cluster(&q.dx, t, d, 2 * blocks(f), sms);
         plan_cluster(&q.dw_gu, 2 * f, d, blocks(t), sms);
         plan_cluster(&q.dw_down, d, f, blocks(t), sms);
         // the two weight gradients are sums over the same rows: in one launch their tiles fill the last round together
         // (8192 x 1024 x 2816: 134 us apart)
-        q.dw_both = plan_gemm(2 * f, d, blocks(t), false, false, sms, d, f);
+        q.dw_both = plan_gemm(2 * f, d, blocks(t), lb::kEpiStore, false, sms, d, f);
         q.together = q.dw_both.us < q.dw_gu.us + q.dw_down.us;
         need(q.dx, t, d);
         need(q.dw_gu, 2 * f, d);

@@ -9,11 +9,15 @@
 //
 // A tile is 128 rows per CTA (CG = 2: 256 rows over a pair of CTAs, each of which holds half of B's tile and so stages half
 // as much per multiply) by BN columns. Warp 0 issues the TMA loads into a ring of stages, warp 1 the multiplies, the others
-// empty the accumulators; two accumulators in TMEM let the epilogue of one tile run under the multiplies of the next.
+// empty the accumulators; two accumulators in TMEM let the epilogue of one tile run under the multiplies of the next. The pair's
+// tile of 512 columns (two multiplies side by side) has one accumulator, all of TMEM, and reads a quarter less per multiply:
+// alone it is as fast (2816 x 1024 weight gradients 83 us against 86), but a training pass in a row, at the power cap, gains
+// 3-4 % (8192 x 1024 x 2816: 397 -> 383 us, 16411 x 1536 x 4096: 1561 -> 1503). Where the tiles no longer fill the GPU it
+// loses (2048 x 1024 x 2816: 162 against 128).
 //
 // What bounds it, for 8192 rows of 1024 with 2816 hidden columns: the pair's tile needs 64 bytes per clock and SM from L2, which
-// serves the launch at 10-14 TB/s, and the power cap; 1.43 PFLOP/s for the input's gradient, 1.47 for both weight gradients,
-// 1.27 down, 1.28 for the gated projections without and 1.14 with the kept factors (whose 138 MB of writes share L2 with the
+// serves the launch at 10-14 TB/s, and the power cap; 1.58 PFLOP/s for the input's gradient, 1.70 for both weight gradients,
+// 1.34 down (one round of 64 tiles on 74 pairs), 1.28 for the gated projections without and 1.14 with the kept factors (whose 138 MB of writes share L2 with the
 // operands; without any epilogue, in a copy made for the measurement, 1.46-1.69). The single CTA's 128 x 256 tile reached 1.23
 // for the input's gradient, 128 x 128 0.81.
 #pragma once
@@ -35,7 +39,10 @@ struct GemmShape {
     static constexpr int kEpiWarps = kGated ? BN / 16 : 4;
     static constexpr int kThreads = 64 + 32 * kEpiWarps;
     static constexpr int kABytes = kGemmM * 128;
-    static constexpr int kBRows = BN / CG;                           // of B's tile in this CTA
+    // a tile of 512 columns is two multiplies side by side; its accumulator takes all of TMEM
+    static constexpr int kParts = BN > 256 ? BN / 256 : 1, kAccs = BN > 256 ? 1 : 2;
+    static constexpr int kPartRows = BN / kParts / CG;               // of B's tile in this CTA, per part
+    static constexpr int kBRows = kParts * kPartRows;
     static constexpr int kStageBytes = kABytes + kBRows * 128;
     static constexpr int kBuf = kGated ? 2048 : 4096;                // result box of a warp, two of them
     static constexpr int kStaging = kEpiWarps * 2 * kBuf;
@@ -43,8 +50,8 @@ struct GemmShape {
     static constexpr int kFit = (kGemmMaxSmem - kTail - kStaging) / kStageBytes;
     static constexpr int kStages = kFit < 8 ? kFit : 8;
     static constexpr int kSmem = kTail + kStaging + kStages * kStageBytes;
-    static constexpr int kCols = 2 * BN < 32 ? 32 : 2 * BN;          // TMEM columns: two accumulators (a power of two)
-    static_assert(kStages >= 2 && 2 * BN <= 512 && (BN & (BN - 1)) == 0, "tile does not fit");
+    static constexpr int kCols = kAccs * BN;                         // TMEM columns (a power of two)
+    static_assert(kStages >= 2 && kCols >= 32 && kCols <= 512 && (BN & (BN - 1)) == 0 && (kParts == 1 || EPI == kEpiStore), "tile does not fit");
 };
 
 // ---------------------------------------------------------------------------------------------------------
@@ -243,6 +250,14 @@ __device__ __forceinline__ TileAt tile_at(int t, const GemmParams &p) {
     return a;
 }
 
+// the parts of a tile that hold columns of the result
+template <typename Sh, bool A_MN, int BN>
+__device__ __forceinline__ int parts_of(const TileAt &at, const GemmParams &p) {
+    if constexpr (Sh::kParts == 1) return 1;
+    const int left = (A_MN && at.product ? p.n2 : p.n) - at.n * BN;
+    return left <= BN / 2 ? 1 : 2;
+}
+
 template <int CG, int BN, int EPI, bool A_MN, bool B_MN, int ACT>
 __global__ void __launch_bounds__(GemmShape<CG, BN, EPI>::kThreads, 1)
 gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
@@ -296,13 +311,14 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
                 const TileAt at = tile_at(t, p);
                 const int kb0 = (int)((long long)blocks * at.split / p.splits), kb1 = (int)((long long)blocks * (at.split + 1) / p.splits);
                 const int m0 = (at.m * CG + (int)rank) * kGemmM;
-                const int n0 = EPI == kEpiGate ? at.n * (BN / 2) : at.n * BN + (int)rank * Sh::kBRows;
+                const int n0 = EPI == kEpiGate ? at.n * (BN / 2) : at.n * BN + (int)rank * Sh::kPartRows;
+                const int parts = parts_of<Sh, A_MN, BN>(at, p);
                 for (int kb = kb0; kb < kb1; ++kb) {
                     if (!(ok = mbar_wait(empty + 8 * s, ph ^ 1, wc, kDevWaitEmpty))) break;
                     const int half = kb >= p.kblocks, k0 = (kb - half * p.kblocks) * kGemmK;
                     const int seg = A_MN ? at.product : half;
                     const uint32_t sa = base + s * Sh::kStageBytes, sb = sa + Sh::kABytes, bar = lead_full + 8 * s;
-                    if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, CG * Sh::kStageBytes);
+                    if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, CG * (Sh::kStageBytes - (Sh::kParts - parts) * Sh::kPartRows * 128));
                     if (p.test_skip_item != 0 && blockIdx.x == 0 && issued + 1 == p.test_skip_item) {
                         // test hook: this copy never comes
                     } else if constexpr (!A_MN) {
@@ -319,10 +335,12 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
                             tma_tile<CG>(sb + (BN / 2) * 128, &maps.b[1], bar, k0, n0);
                         }
                     } else if constexpr (!B_MN) {
-                        tma_tile<CG>(sb, &maps.b[seg], bar, k0, n0);
+                        for (int q = 0; q < parts; ++q) tma_tile<CG>(sb + q * Sh::kPartRows * 128, &maps.b[seg], bar, k0, n0 + q * 256);
                     } else {
+                        for (int q = 0; q < parts; ++q)
 #pragma unroll
-                        for (int j = 0; j < Sh::kBRows / 64; ++j) tma_tile<CG>(sb + j * 8192, &maps.b[seg], bar, n0 + 64 * j, k0);
+                            for (int j = 0; j < Sh::kPartRows / 64; ++j)
+                                tma_tile<CG>(sb + q * Sh::kPartRows * 128 + j * 8192, &maps.b[seg], bar, n0 + q * 256 + 64 * j, k0);
                     }
                     ++issued;
                     if (++s == ST) { s = 0; ph ^= 1; }
@@ -345,7 +363,7 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
-            constexpr uint32_t idesc = mma_idesc(kGemmM * CG, BN, A_MN, B_MN);
+            constexpr uint32_t idesc = mma_idesc(kGemmM * CG, BN / Sh::kParts, A_MN, B_MN);
             constexpr uint32_t ka = A_MN ? 2048 >> 4 : 32 >> 4, kb_ = B_MN ? 2048 >> 4 : 32 >> 4;   // 16 k further
             int s = 0, acc = 0;
             uint32_t ph = 0, aph = 0;
@@ -353,6 +371,7 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
             for (int t = first; ok && t < tiles; t += step) {
                 const TileAt at = tile_at(t, p);
                 const int kb0 = (int)((long long)blocks * at.split / p.splits), kb1 = (int)((long long)blocks * (at.split + 1) / p.splits);
+                const int parts = parts_of<Sh, A_MN, BN>(at, p);
                 if (!(ok = mbar_wait(tempty + 8 * acc, aph ^ 1, wc, kDevWaitTmem))) break;
                 tc_fence_after();
                 const uint32_t d = tmem + acc * BN;
@@ -361,14 +380,16 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
                     tc_fence_after();
                     const uint32_t sa = base + s * Sh::kStageBytes;
                     const uint64_t da = tile_desc(sa, A_MN, 8192), db = tile_desc(sa + Sh::kABytes, B_MN, 8192);
+                    for (int q = 0; q < parts; ++q)
 #pragma unroll
-                    for (int k = 0; k < kGemmK / 16; ++k) tc_mma<CG>(d, da + k * ka, db + k * kb_, idesc, kb > kb0 || k > 0);
+                        for (int k = 0; k < kGemmK / 16; ++k)
+                            tc_mma<CG>(d + q * 256, da + k * ka, db + q * (Sh::kPartRows * 128 >> 4) + k * kb_, idesc, kb > kb0 || k > 0);
                     tc_commit<CG>(empty + 8 * s);
                     if (++s == ST) { s = 0; ph ^= 1; }
                 }
                 if (!ok) break;
                 tc_commit<CG>(tfull + 8 * acc);
-                if (++acc == 2) { acc = 0; aph ^= 1; }
+                if (++acc == Sh::kAccs) { acc = 0; aph ^= 1; }
             }
             tc_drain<CG>(mdone, p.wait_cycles);
         }
@@ -543,7 +564,7 @@ gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
                     }
                 }
             }
-            if (++acc == 2) { acc = 0; aph ^= 1; }
+            if (++acc == Sh::kAccs) { acc = 0; aph ^= 1; }
         }
         if (lane == 0) bulk_wait_all();
     }

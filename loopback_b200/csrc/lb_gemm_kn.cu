@@ -18,6 +18,7 @@ cudaError_t launch_gemm_kn(int tile, int epilogue, const GemmMaps &maps, const G
         case 0: return pick<1, 128>(epilogue, maps, p, sms, stream);
         case 1: return pick<1, 256>(epilogue, maps, p, sms, stream);
         case 2: return pick<2, 256>(epilogue, maps, p, sms, stream);
+        case 3: return epilogue == kEpiStore ? launch_gemm_t<2, 512, kEpiStore, false, true>(maps, p, sms, stream) : cudaErrorInvalidValue;
     }
     return cudaErrorInvalidValue;
 }

@@ -256,8 +256,8 @@ enum GemmForm : int {
 struct GemmTile {
     int cg, bn;
 };
-constexpr GemmTile kGemmTiles[] = {{1, 128}, {1, 256}, {2, 256}};
-constexpr int kGemmTileCount = 3;
+constexpr GemmTile kGemmTiles[] = {{1, 128}, {1, 256}, {2, 256}, {2, 512}};   // the last: plain products, k not split
+constexpr int kGemmTileCount = 4;
 
 cudaError_t launch_gemm(int tile, int epilogue, int form, const GemmMaps &maps, const GemmParams &p, int sms, cudaStream_t stream);
 // the product of tile shape 0 split along k over clusters of p.splits CTAs (2..8), one tile each (lb_gemm_cluster.cu)

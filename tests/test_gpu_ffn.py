@@ -36,7 +36,7 @@ SIZES = [(128, 64, 128), (128, 128, 256), (256, 256, 512), (1, 8, 8), (1, 64, 64
          (129, 768, 2048), (255, 1000, 136), (257, 264, 520), (300, 8, 1032), (300, 1032, 8), (1000, 512, 1408)]
 
 
-@pytest.mark.parametrize("tile", [1, 2, 3, 4])
+@pytest.mark.parametrize("tile", [1, 2, 3, 4, 5])
 @pytest.mark.parametrize("t,d,f", SIZES)
 def test_training_sizes(t, d, f, tile):
     import loopback_b200._lib as L
@@ -47,7 +47,7 @@ def test_training_sizes(t, d, f, tile):
         L.reset_options()
 
 
-@pytest.mark.parametrize("tile,t", [(1, 1400), (2, 1400), (3, 1400), (4, 700)])
+@pytest.mark.parametrize("tile,t", [(1, 1400), (2, 1400), (3, 1400), (5, 700)])
 @pytest.mark.parametrize("splits", [1, 2, 3, 5, 6, 7, 8])
 def test_splits_along_k(tile, t, splits):
     import loopback_b200._lib as L
@@ -55,6 +55,17 @@ def test_splits_along_k(tile, t, splits):
         L.set_option("ffn_tile", tile)
         L.set_option("ffn_splits", splits)
         _check(t, 264, 1288, seed=splits)
+    finally:
+        L.reset_options()
+
+
+@pytest.mark.parametrize("t,d,f", [(16500, 520, 72), (300, 1544, 4096), (20011, 264, 776)])
+def test_several_wide_tiles_per_pair(t, d, f):
+    """256 x 512 tiles have one accumulator: more tiles than pairs of CTAs, with a last one of one half or less."""
+    import loopback_b200._lib as L
+    try:
+        L.set_option("ffn_tile", 4)
+        _check(t, d, f, seed=t)
     finally:
         L.reset_options()
 
@@ -227,7 +238,7 @@ def test_on_another_stream_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(grads, want))
 
 
-@pytest.mark.parametrize("t,tile", [(300, 1), (300, 3), (300, 4), (40, 0)])
+@pytest.mark.parametrize("t,tile", [(300, 1), (300, 3), (300, 4), (300, 5), (40, 0)])
 def test_a_wait_that_runs_out_unwinds_and_reports(t, tile):
     """The products' waits are bounded. With the limit at about a millisecond and the hook that leaves out one tile copy of the
     first CTA, its multiplies give up, everybody unwinds, the kernel returns and the device error word names a wait; the next
