@@ -69,7 +69,8 @@ def block_residual(x: torch.Tensor, y: torch.Tensor, weight=None, *, gate=None, 
     gate         None, (d,) per channel, (..., 1) per token or x's shape
     scale        a number, or a tensor of one element (learned)
     next_weight  (d,) of the norm of out; its statistics come from out before it is rounded to its storage type
-    p, rng       dropout of the (normed) block output, as in `dropout`, drawn over x's elements
+    p, rng       dropout of the (normed) block output, as in `dropout`, drawn over x's elements; without `weight`, what y holds
+                 where it is dropped reaches neither the results nor a gradient
     Per-channel parameters are in x's type or fp32, gates per token or element in x's. Differentiable (once) in every tensor."""
     t = _threshold("block_residual", p) if p else 0
     pair, seed, offset = _rng_args("block_residual", rng) if t else (None, 0, 0)
